@@ -259,9 +259,89 @@ int cs2d_bwd_noalloc(const cs2d_problem *p, const void *dout, int64_t dout_bs, i
                      float *dC, float *dD, float *ddelta_bias, float *dA_decay, void *stream);
 
 /*
+ * Gated linear recurrence over tokens (no counterpart in the reference): per batch row and channel
+ *     h[t] = a[t] * h[t-1] + b[t],   y[t] = h[t],   h[-1] = h0
+ * with a from the gate by `form` (CS2D_GATE_SIGMOID: 1 / (1 + exp(-gate)), CS2D_GATE_LOG: exp(gate),
+ * CS2D_GATE_DIRECT: gate) and b = u, or (1 - a) * u where `weighted` is set.  The state is fp32 throughout; y is
+ * rounded to the input type once per element.  Factors above one are allowed as long as the product of
+ * 256 consecutive ones stays inside the range of fp32.
+ *
+ * u, gate (batch, length, dim) of io_dtype, channel stride 1, other strides in elements.  h0 (states, dim) fp32, rows
+ * h0_bs apart, or NULL (zeros).  Without `offsets` there are `batch` states.  With them batch is 1 and `offsets`
+ * (device, n_seq + 1 ascending int32, or int64 where offsets64 is set) cuts the rows into n_seq sequences
+ * [offsets[s], offsets[s+1]) with a state each; a sequence may be empty (its h0 passes through).  Rows of no sequence
+ * are not read; y, du and dgate are zero there.  Offsets that do not ascend or leave the tensor set bit 3 of the status
+ * word; the outputs are then invalid, nothing outside of them is touched.
+ */
+typedef enum { CS2D_GATE_SIGMOID = 0, CS2D_GATE_LOG = 1, CS2D_GATE_DIRECT = 2 } cs2d_gate_form;
+typedef struct {
+    int32_t batch, dim, io_dtype, form, weighted;
+    int32_t n_seq, offsets64;
+    int64_t length;
+    const void *u;    int64_t u_bs, u_ls;
+    const void *gate; int64_t gate_bs, gate_ls;
+    const float *h0;  int64_t h0_bs;   /* may be NULL */
+    const void *offsets;               /* may be NULL */
+} cs2d_gscan;
+
+/*
+ * Bytes of the buffer between forward and backward: checkpoints of the state every 128 rows and, with offsets, 8 bytes
+ * per row.  keep = 0: what a forward needs that no backward will follow.  At least 16; 0 for an invalid problem.
+ */
+size_t cs2d_gscan_saved_bytes(const cs2d_gscan *p, int keep);
+
+/*
+ * Forward: y (batch, length, dim) of io_dtype, channel stride 1; h_last (states, dim) fp32, dense; saved as above,
+ * 16-byte aligned.  The same bits on every run.
+ */
+int cs2d_gscan_fwd(const cs2d_gscan *p, void *y, int64_t y_bs, int64_t y_ls, float *h_last, void *saved, int keep, void *stream);
+
+/*
+ * Backward, from what the forward of the same problem saved (it is only read): dy like u, dh_last (states, dim) fp32, rows
+ * dh_last_bs apart, or NULL (zeros); du, dgate (batch, length, dim) of io_dtype, dense; dh0 (states, dim) fp32, dense, or NULL.
+ * Everything is written, nothing accumulated; the same bits on every run.
+ */
+int cs2d_gscan_bwd(const cs2d_gscan *p, const void *dy, int64_t dy_bs, int64_t dy_ls, const float *dh_last, int64_t dh_last_bs,
+                   const void *saved, void *du, void *dgate, float *dh0, void *stream);
+
+/*
+ * One token: u, gate, y (batch, dim) (u_ls, gate_ls, length, offsets, h0 are not used); the state h (batch, dim) fp32, rows
+ * h_bs apart, is read and overwritten.
+ */
+int cs2d_gscan_step(const cs2d_gscan *p, void *y, int64_t y_bs, float *h, int64_t h_bs, void *stream);
+
+/*
+ * Layer norm over the channels of a row, with an optional SiLU gate behind it (no counterpart in the reference):
+ *     y = ((x - mean) / sqrt(var + eps) * weight + bias) * silu(gate)
+ * Row (o, i), 0 <= o < outer, 0 <= i < inner, channel d is x[o * x_os + i * x_is + d * x_cs]; x_cs (rows of tokens) or x_is
+ * (channel-major images) must be 1.  gate: channel stride 1, or NULL.  weight, bias (dim) of param_dtype (fp32 or the
+ * input type), dense, or NULL (ones, zeros).  y (outer, inner, dim) of io_dtype, dense.  stats (outer * inner, 2) fp32 receives mean
+ * and 1 / sqrt(var + eps) for the backward, or NULL.  Sums and statistics are fp32, the variance that of the centred values.
+ */
+typedef struct {
+    int32_t dim, io_dtype, param_dtype;
+    float eps;
+    int64_t outer, inner;
+    const void *x;    int64_t x_os, x_is, x_cs;
+    const void *gate; int64_t g_os, g_is;   /* may be NULL */
+    const void *weight, *bias;              /* may be NULL */
+} cs2d_norm;
+int cs2d_norm_fwd(const cs2d_norm *p, void *y, float *stats, void *stream);
+
+/*
+ * Backward: dy like the gate in strides; scratch of cs2d_norm_bwd_scratch_bytes(p) bytes, 16-byte aligned, private to the call;
+ * dx with the strides given (dx_cs or dx_is 1), dgate (outer, inner, dim) dense (NULL without a gate), dweight and dbias (dim) of param_dtype,
+ * each may be NULL.  Written, not accumulated; the sums over the rows are fp32 in a fixed order: the same bits on every run.
+ */
+size_t cs2d_norm_bwd_scratch_bytes(const cs2d_norm *p);
+int cs2d_norm_bwd(const cs2d_norm *p, const void *dy, int64_t dy_os, int64_t dy_is, const float *stats, void *scratch, void *dx,
+                  int64_t dx_os, int64_t dx_is, int64_t dx_cs, void *dgate, void *dweight, void *dbias, void *stream);
+
+/*
  * Reads and clears the device-side status word of the current device
  * (synchronises with the device).  0 = no kernel reported a problem; nonzero =
- * a kernel gave up on a bounded wait (bit 0: for one of its asynchronous copies,
+ * a kernel met sequence offsets that it cannot follow (bit 3), or
+ * gave up on a bounded wait (bit 0: for one of its asynchronous copies,
  * bit 1: for the tiles its staging warps hand to its compute warps, bit 2: for a
  * block of another row worker) and
  * returned early, so the outputs of the calls since the last check are invalid

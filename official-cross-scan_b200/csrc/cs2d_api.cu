@@ -10,6 +10,7 @@
 #include "cs2d_blk.cuh"
 #include "cs2d_pair.cuh"
 #include "cs2d_common.cuh"
+#include "cs2d_host.h"
 
 namespace cs2d {
 cudaError_t launch_fwd(const Dev &P, int L, int grid, cudaStream_t st);
@@ -32,7 +33,7 @@ size_t bwd_smem_bytes(int L, int CG, int NPp, int CT, bool acc, int W, int es, i
 static __device__ int g_cs2d_status = 0;  // see ERR_* in cs2d_status.h
 
 // Device address of the status word on the current device (looked up once per device).
-static int *status_ptr() {
+int *status_ptr() {
     static int *ptr[64] = {};
     int dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return nullptr;
@@ -44,7 +45,9 @@ static int *status_ptr() {
 static thread_local char g_err[512] = "";
 static std::atomic<int64_t> g_launches{0};
 
-__attribute__((format(printf, 2, 3))) static int fail(int code, const char *fmt, ...) {
+void count_launches(int n) { g_launches.fetch_add(n); }
+
+int fail(int code, const char *fmt, ...) {
     va_list ap;
     va_start(ap, fmt);
     vsnprintf(g_err, sizeof(g_err), fmt, ap);

@@ -12,6 +12,7 @@
 // problems take one allocation and one fill for all of these and the scratch (see BwdBuffers).  The backward
 // runs on a thread of the autograd engine that has just been woken: every call of the tensor library costs
 // twice there what it costs in a warm loop (measured 45 us for what takes 22 us on the calling thread).
+#include <c10/cuda/CUDAGraphsC10Utils.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <cuda_runtime_api.h>
@@ -442,6 +443,8 @@ Tensor py_cross(const Tensor &u, const Tensor &delta, const Tensor &A, const Ten
     return y.scalar_type() == u.scalar_type() ? y : y.to(u.scalar_type());
 }
 
+#include "cs2d_torch_seq.h"
+
 // the two halves of the four-corner operator on their own: (y fp32, state), then the gradients
 std::tuple<Tensor, OptT> py_cross_fwd(const Tensor &u, const Tensor &delta, const Tensor &A, const Tensor &B, const Tensor &C, const Tensor &w,
                                       const OptT &D, const OptT &bias, bool softplus, bool keep_state, const OptT &decay, bool serial) {
@@ -466,13 +469,16 @@ std::vector<OptT> py_cross_bwd(const Tensor &u, const Tensor &delta, const Tenso
 }  // namespace
 
 PYBIND11_MODULE(_native, m) {
-    m.doc() = "native host path of the cs2d operators (see cs2d/ops.py and cs2d/cross.py)";
+    m.doc() = "native host path of the cs2d operators (see cs2d/ops.py, cs2d/cross.py, cs2d/seq.py and cs2d/norm.py)";
     m.def("problem", &py_problem);
     m.def("fwd", &py_fwd, py::call_guard<py::gil_scoped_release>());
     m.def("fwd_only", &py_fwd_only, py::call_guard<py::gil_scoped_release>());
     m.def("bwd", &py_bwd, py::call_guard<py::gil_scoped_release>());
     m.def("scan", &py_scan, py::call_guard<py::gil_scoped_release>());
     m.def("cross", &py_cross, py::call_guard<py::gil_scoped_release>());
+    m.def("gated_scan", &py_gated_scan, py::call_guard<py::gil_scoped_release>());
+    m.def("gated_step", &py_gated_step, py::call_guard<py::gil_scoped_release>());
+    m.def("layer_norm", &py_layer_norm, py::call_guard<py::gil_scoped_release>());
     m.def("cross_fwd", &py_cross_fwd, py::call_guard<py::gil_scoped_release>());
     m.def("cross_bwd", &py_cross_bwd, py::call_guard<py::gil_scoped_release>());
 }
