@@ -285,7 +285,7 @@ typedef struct {
 } cs2d_gscan;
 
 /*
- * Bytes of the buffer between forward and backward: checkpoints of the state every 128 rows and, with offsets, 8 bytes
+ * Bytes of the buffer between forward and backward: checkpoints of the state every 32 rows and, with offsets, 8 bytes
  * per row.  keep = 0: what a forward needs that no backward will follow.  At least 16; 0 for an invalid problem.
  */
 size_t cs2d_gscan_saved_bytes(const cs2d_gscan *p, int keep);

@@ -16,29 +16,27 @@
 namespace cs2d {
 
 // ---- gated scan ------------------------------------------------------------------------------------------
-// Units of work: a batch row and a block of 32 lanes x V channels.  Rows are tokens.
+// Units of work: a batch row and a block of channels.  Rows are tokens.
 struct GScan {
-    int batch, dim, nblk, nseq, form, weighted, off64, nck;
-    int64_t units, length;
+    int batch, dim, nblk, nseq, form, weighted, off64;
+    int64_t units, length, nck;
     const void *u, *gate, *dy, *offsets;
     const float *h0, *dlast;
     void *y, *du, *dgate;
-    float *last, *dh0, *ckpt, *h;   // ckpt: [batch][nck][dim], the state before rows CK, 2 CK, ...; h: the step's state
+    float *last, *dh0, *ckpt, *h;   // ckpt: [batch][nck][dim], the state before rows GS_CK, 2 GS_CK, ...; h: the step's state
     int2 *map;                      // packed: per row the sequence that starts there and the one that ends there (SEQ_NONE, SEQ_OUTSIDE)
     int64_t u_bs, u_ls, g_bs, g_ls, dy_bs, dy_ls, y_bs, y_ls, h0_bs, h_bs, dlast_bs;
+    int io, io_out;                 // how rows are read and written: GS_CHUNKS, GS_WORDS, GS_ELEMENTS
     int *status;
 };
 enum { SEQ_NONE = -1, SEQ_OUTSIDE = -2 };
+enum { GS_CHUNKS = 0, GS_WORDS = 1, GS_ELEMENTS = 2 };   // 16 bytes, a lane's two channels, one channel at a time
 
-constexpr int GS_WARPS = 16;   // warps of a CTA
-constexpr int GS_TW = 16;      // rows of a warp, forward
-constexpr int GS_TWB = 8;      // rows of a warp, backward
-constexpr int GS_CK = GS_WARPS * GS_TWB;   // rows between two checkpoints: the backward's tile
+constexpr int GS_CK = 32;       // rows between two checkpoints; the backward's tiles are multiples of it
 
-// Channels of a lane: one 32-bit word of them where every row starts on a word, one channel otherwise.
 cudaError_t launch_gscan_map(const GScan &P, cudaStream_t st);
-cudaError_t launch_gscan_fwd(const GScan &P, int dt, bool words, cudaStream_t st);
-cudaError_t launch_gscan_bwd(const GScan &P, int dt, bool words, cudaStream_t st);
+cudaError_t launch_gscan_fwd(const GScan &P, int dt, cudaStream_t st);
+cudaError_t launch_gscan_bwd(const GScan &P, int dt, cudaStream_t st);
 cudaError_t launch_gscan_step(const GScan &P, int dt, cudaStream_t st);
 
 // ---- layer norm --------------------------------------------------------------------------------------------
@@ -102,8 +100,19 @@ template <int DT, int V> struct Pack {
 };
 
 // ---- the gate: its factor a and c = 1 - a, each to a few units of its own last place ---------------------------
-template <bool FULL> __device__ __forceinline__ float exp_of(float x) { return FULL ? expf(x) : __expf(x); }
-template <bool FULL> __device__ __forceinline__ float over(float x, float y) { return FULL ? x / y : __fdividef(x, y); }
+// FULL: for fp32 inputs; 16-bit ones take the hardware's exponential and reciprocal (denormals flushed).
+__device__ __forceinline__ float ex2_fast(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ float rcp_fast(float x) {
+    float y;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+template <bool FULL> __device__ __forceinline__ float exp_of(float x) { return FULL ? expf(x) : ex2_fast(x * 1.4426950408889634f); }
+template <bool FULL> __device__ __forceinline__ float over(float x, float y) { return FULL ? x / y : x * rcp_fast(y); }
 
 // a = 1 / (1 + exp(-g)).  The smaller of a and c is computed, the larger one is one less it: both keep their own digits, and a
 // product of thousands of factors next to one does not drift (an approximate reciprocal next to one would).
@@ -114,21 +123,21 @@ template <bool FULL> __device__ __forceinline__ void gate_sigmoid(float g, float
     c = g > 0.f ? small : large;
 }
 // a = exp(g), c = -expm1(g).  Near zero the Taylor series of expm1 (next term below 2e-8 of it for |g| <= 0.35) gives both.
-__device__ __forceinline__ void gate_log(float g, float &a, float &c) {
+template <bool FULL> __device__ __forceinline__ void gate_log(float g, float &a, float &c) {
     float p = 1.f / 5040.f;
     p = fmaf(p, g, 1.f / 720.f);
     p = fmaf(p, g, 1.f / 120.f);
     p = fmaf(p, g, 1.f / 24.f);
     p = fmaf(p, g, 1.f / 6.f);
     p = fmaf(p, g, 0.5f);
-    const float m = fmaf(p * g, g, g), e = expf(g);
+    const float m = fmaf(p * g, g, g), e = exp_of<FULL>(g);
     const bool near = fabsf(g) <= 0.35f;
     a = near ? 1.f + m : e;
     c = near ? -m : 1.f - e;
 }
 template <int FORM, bool FULL> __device__ __forceinline__ void gate_values(float g, float &a, float &c) {
     if constexpr (FORM == CS2D_GATE_SIGMOID) gate_sigmoid<FULL>(g, a, c);
-    else if constexpr (FORM == CS2D_GATE_LOG) gate_log(g, a, c);
+    else if constexpr (FORM == CS2D_GATE_LOG) gate_log<FULL>(g, a, c);
     else { a = g; c = 1.f - g; }
 }
 template <bool FULL> __device__ __forceinline__ float sigmoid(float z) {

@@ -13,33 +13,33 @@ static int validate(const cs2d_gscan *p, bool step) {
     if (p->form < CS2D_GATE_SIGMOID || p->form > CS2D_GATE_DIRECT) return fail(CS2D_ERR_INVALID, "unknown form of the gate: %d", p->form);
     if (!p->u || !p->gate) return fail(CS2D_ERR_INVALID, "u and gate must be given");
     if (step) return CS2D_OK;
-    if (p->length > ((int64_t)1 << 38)) return fail(CS2D_ERR_UNSUPPORTED, "more than 2^38 tokens");
+    if (p->length > (1 << 30)) return fail(CS2D_ERR_UNSUPPORTED, "more than 2^30 tokens in a row");
     if (p->offsets && p->batch != 1) return fail(CS2D_ERR_INVALID, "with offsets the batch is 1");
     if (p->offsets && p->n_seq < 0) return fail(CS2D_ERR_INVALID, "n_seq must not be negative");
     return CS2D_OK;
 }
-// Every row starts on a 32-bit word: lanes may take two 16-bit channels at a time.
-static bool on_words(std::initializer_list<const void *> ptrs, std::initializer_list<int64_t> strides) {
+// Every row starts on a multiple of `bytes`, and so does what is behind its last channel.
+static bool aligned(int bytes, int es, int dim, std::initializer_list<const void *> ptrs, std::initializer_list<int64_t> strides) {
     for (const void *p : ptrs)
-        if (reinterpret_cast<uintptr_t>(p) % 4) return false;
+        if (reinterpret_cast<uintptr_t>(p) % bytes) return false;
     for (int64_t s : strides)
-        if (s % 2) return false;
-    return true;
+        if (s * es % bytes) return false;
+    return dim * (int64_t)es % bytes == 0;
+}
+static int how_moved(int es, int dim, std::initializer_list<const void *> ptrs, std::initializer_list<int64_t> strides) {
+    return aligned(16, es, dim, ptrs, strides) ? GS_CHUNKS : aligned(4, es, dim, ptrs, strides) ? GS_WORDS : GS_ELEMENTS;
 }
 static size_t map_bytes(const cs2d_gscan *p) { return p->offsets ? ((size_t)p->length * 8 + 15) / 16 * 16 : 0; }
 static int64_t checkpoints(const cs2d_gscan *p) { return (p->length - 1) / GS_CK; }
-static int fill(GScan &d, const cs2d_gscan *p, void *saved, bool words) {
+static int fill(GScan &d, const cs2d_gscan *p, void *saved) {
     d = GScan{};
     d.batch = p->batch; d.dim = p->dim; d.form = p->form; d.weighted = p->weighted != 0; d.length = p->length;
     d.nseq = p->offsets ? p->n_seq : 0; d.offsets = p->offsets; d.off64 = p->offsets64;
-    const int per = 32 * (p->io_dtype == CS2D_F32 || !words ? 1 : 2);
-    d.nblk = (p->dim + per - 1) / per;
-    d.units = (int64_t)p->batch * d.nblk;
-    if (d.units > INT32_MAX) return fail(CS2D_ERR_UNSUPPORTED, "batch times channels is too large");
+    if ((int64_t)p->batch * ((p->dim + 15) / 16) > INT32_MAX) return fail(CS2D_ERR_UNSUPPORTED, "batch times channels is too large");
     d.u = p->u; d.u_bs = p->u_bs; d.u_ls = p->u_ls;
     d.gate = p->gate; d.g_bs = p->gate_bs; d.g_ls = p->gate_ls;
     d.h0 = p->h0; d.h0_bs = p->h0_bs;
-    d.nck = (int)checkpoints(p);
+    d.nck = checkpoints(p);
     d.map = p->offsets ? (int2 *)saved : nullptr;
     d.ckpt = (float *)((char *)saved + map_bytes(p));
     d.status = status_ptr();
@@ -88,27 +88,31 @@ size_t cs2d_gscan_saved_bytes(const cs2d_gscan *p, int keep) {
 int cs2d_gscan_fwd(const cs2d_gscan *p, void *y, int64_t y_bs, int64_t y_ls, float *h_last, void *saved, int keep, void *stream) {
     if (const int rc = validate(p, false)) return rc;
     if (!y || !saved || (!h_last && !(p->offsets && p->n_seq == 0))) return fail(CS2D_ERR_INVALID, "y, h_last and saved must be given");
-    const bool words = p->dim % 2 == 0 && on_words({p->u, p->gate, y}, {p->u_bs, p->u_ls, p->gate_bs, p->gate_ls, y_bs, y_ls});
     GScan d;
-    if (const int rc = fill(d, p, saved, words)) return rc;
+    if (const int rc = fill(d, p, saved)) return rc;
+    const int es = p->io_dtype == CS2D_F32 ? 4 : 2;
+    d.io = how_moved(es, p->dim, {p->u, p->gate}, {p->u_bs, p->u_ls, p->gate_bs, p->gate_ls});
+    d.io_out = how_moved(es, p->dim, {y}, {y_bs, y_ls});
     d.y = y; d.y_bs = y_bs; d.y_ls = y_ls; d.last = h_last;
     if (!keep) d.ckpt = nullptr;
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
     if (d.map)
         if (const int rc = launched(launch_gscan_map(d, st), 1)) return rc;
-    return launched(launch_gscan_fwd(d, p->io_dtype, words, st), 1);
+    return launched(launch_gscan_fwd(d, p->io_dtype, st), 1);
 }
 
 int cs2d_gscan_bwd(const cs2d_gscan *p, const void *dy, int64_t dy_bs, int64_t dy_ls, const float *dh_last, int64_t dh_last_bs,
                    const void *saved, void *du, void *dgate, float *dh0, void *stream) {
     if (const int rc = validate(p, false)) return rc;
     if (!dy || !saved || !du || !dgate) return fail(CS2D_ERR_INVALID, "dy, saved, du and dgate must be given");
-    const bool words = p->dim % 2 == 0 && on_words({p->u, p->gate, dy, du, dgate}, {p->u_bs, p->u_ls, p->gate_bs, p->gate_ls, dy_bs, dy_ls});
     GScan d;
-    if (const int rc = fill(d, p, const_cast<void *>(saved), words)) return rc;
+    if (const int rc = fill(d, p, const_cast<void *>(saved))) return rc;
+    const int es = p->io_dtype == CS2D_F32 ? 4 : 2;
+    d.io = how_moved(es, p->dim, {p->u, p->gate, dy}, {p->u_bs, p->u_ls, p->gate_bs, p->gate_ls, dy_bs, dy_ls});
+    d.io_out = how_moved(es, p->dim, {du, dgate}, {p->length * p->dim, p->dim});
     d.dy = dy; d.dy_bs = dy_bs; d.dy_ls = dy_ls; d.dlast = dh_last; d.dlast_bs = dh_last_bs;
     d.du = du; d.dgate = dgate; d.y_bs = p->length * p->dim; d.y_ls = p->dim; d.dh0 = dh0;
-    return launched(launch_gscan_bwd(d, p->io_dtype, words, static_cast<cudaStream_t>(stream)), 1);
+    return launched(launch_gscan_bwd(d, p->io_dtype, static_cast<cudaStream_t>(stream)), 1);
 }
 
 int cs2d_gscan_step(const cs2d_gscan *p, void *y, int64_t y_bs, float *h, int64_t h_bs, void *stream) {

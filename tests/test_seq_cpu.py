@@ -57,13 +57,13 @@ def _gscan(**over):
 
 def test_gated_scan_sizes():
     L = _lib_with_types()
-    # checkpoints before rows 128, 256, ... 896 of two batch rows; 8 bytes per row with offsets; never nothing
-    assert L.cs2d_gscan_saved_bytes(ctypes.byref(_gscan()), 1) == 2 * 7 * 64 * 4
+    # checkpoints before rows 32, 64, ... 992 of two batch rows; 8 bytes per row with offsets; never nothing
+    assert L.cs2d_gscan_saved_bytes(ctypes.byref(_gscan()), 1) == 2 * 31 * 64 * 4
     assert L.cs2d_gscan_saved_bytes(ctypes.byref(_gscan()), 0) == 16
-    assert L.cs2d_gscan_saved_bytes(ctypes.byref(_gscan(length=128)), 1) == 16
-    assert L.cs2d_gscan_saved_bytes(ctypes.byref(_gscan(length=129)), 1) == 2 * 64 * 4
+    assert L.cs2d_gscan_saved_bytes(ctypes.byref(_gscan(length=32)), 1) == 16
+    assert L.cs2d_gscan_saved_bytes(ctypes.byref(_gscan(length=33)), 1) == 2 * 64 * 4
     p = _gscan(batch=1, offsets=256, n_seq=3)
-    assert L.cs2d_gscan_saved_bytes(ctypes.byref(p), 1) == 8 * 1000 + 7 * 64 * 4
+    assert L.cs2d_gscan_saved_bytes(ctypes.byref(p), 1) == 8 * 1000 + 31 * 64 * 4
     assert L.cs2d_gscan_saved_bytes(ctypes.byref(p), 0) == 8 * 1000
 
 
