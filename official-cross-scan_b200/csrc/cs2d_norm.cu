@@ -1,14 +1,13 @@
-// Layer norm over the channels of a row, with an optional SiLU gate behind it:
-//   xh = (x - mean) / sqrt(var + eps)    n = xh w + b    y = n silu(z)
-//   dn = dy silu(z)   t = dn w   dx = (t - mean(t) - xh mean(t xh)) / sqrt(var + eps)   dz = dy n silu'(z)
-//   dw = sum over rows of dn xh   db = sum over rows of dn
-// Sums and statistics in 32 bits; the variance is that of the centred values.
-#include "cs2d_seq.cuh"
+// Layer norm: how rows are laid over lanes, launches, the sum over slots; rows too wide for registers.  See cs2d_norm.cuh.
+#include "cs2d_norm.cuh"
 
 namespace cs2d {
 
 namespace {
 
+using nm::param;
+
+// ---- rows of more channels than a CTA holds in registers: a warp per row, which reads it again for every step ---------
 constexpr int NW = 8;   // warps of a CTA
 
 __device__ __forceinline__ float warp_sum(float v) {
@@ -16,12 +15,7 @@ __device__ __forceinline__ float warp_sum(float v) {
     for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(~0u, v, o);
     return v;
 }
-__device__ __forceinline__ float param(const void *p, int dt, int i, float none) {
-    if (!p) return none;
-    return dt == CS2D_F32 ? ((const float *)p)[i] : dt == CS2D_F16 ? __half2float(((const __half *)p)[i]) : __bfloat162float(((const __nv_bfloat16 *)p)[i]);
-}
-
-template <int DT> __global__ void __launch_bounds__(NW * 32) norm_fwd(const Norm P) {
+template <int DT> __global__ void __launch_bounds__(NW * 32) wide_fwd(const Norm P) {
     using T = typename Elem<DT>::T;
     const int lane = threadIdx.x & 31;
     const int64_t row = (int64_t)blockIdx.x * NW + (threadIdx.x >> 5);
@@ -49,7 +43,7 @@ template <int DT> __global__ void __launch_bounds__(NW * 32) norm_fwd(const Norm
     }
 }
 
-template <int DT> __global__ void __launch_bounds__(NW * 32) norm_bwd(const Norm P) {
+template <int DT> __global__ void __launch_bounds__(NW * 32) wide_bwd(const Norm P) {
     using T = typename Elem<DT>::T;
     constexpr bool FULL = DT == CS2D_F32;
     const int lane = threadIdx.x & 31;
@@ -86,7 +80,7 @@ template <int DT> __global__ void __launch_bounds__(NW * 32) norm_bwd(const Norm
 }
 
 // the parameters' gradients: rows in `parts` runs, a thread per channel
-template <int DT> __global__ void __launch_bounds__(NW * 32) norm_part(const Norm P) {
+template <int DT> __global__ void __launch_bounds__(NW * 32) wide_part(const Norm P) {
     using T = typename Elem<DT>::T;
     const int d = blockIdx.x * NW * 32 + threadIdx.x;
     if (d >= P.dim) return;
@@ -105,6 +99,7 @@ template <int DT> __global__ void __launch_bounds__(NW * 32) norm_part(const Nor
     P.part[(int64_t)blockIdx.y * 2 * P.dim + d] = w;
     P.part[((int64_t)blockIdx.y * 2 + 1) * P.dim + d] = b;
 }
+// ---- the parameters' gradients from their slots ------------------------------------------------------------------
 __device__ __forceinline__ void put(void *p, int dt, int i, float v) {
     if (!p) return;
     if (dt == CS2D_F32) ((float *)p)[i] = v;
@@ -126,33 +121,89 @@ __global__ void __launch_bounds__(NW * 32) norm_join(const Norm P) {
     else put(P.dbias, P.wtype, i - P.dim, v);
 }
 
-template <int DT> cudaError_t bwd(const Norm &P, cudaStream_t st) {
-    norm_bwd<DT><<<(unsigned)((P.rows + NW - 1) / NW), NW * 32, 0, st>>>(P);
-    if (!P.dweight && !P.dbias) return cudaGetLastError();
-    norm_part<DT><<<dim3((P.dim + NW * 32 - 1) / (NW * 32), P.parts), NW * 32, 0, st>>>(P);
-    norm_join<<<(2 * P.dim + 31) / 32, NW * 32, 0, st>>>(P);
+
+// Lanes of a row and vectors of a lane: the fewest places for the row's vectors, of equal ones the fewest lanes (fewer shuffles).
+bool lanes_of(int dim, int v, int dt, int *T, int *nv) {
+    static const int narrow[] = {1, 2, 3, 0}, f32[] = {1, 2, 3, 6, 0}, single[] = {4, 12, 24, 0};
+    const int *set = v == 1 ? single : dt == CS2D_F32 ? f32 : narrow;
+    const int nvec = dim / v;
+    int best = 0;
+    for (int t = 1; t <= nm::NT; t <<= 1)
+        for (const int *s = set; *s; ++s) {
+            if (t * *s < nvec) continue;
+            if (!best || t * *s < best) { best = t * *s; *T = t; *nv = *s; }
+            break;
+        }
+    return best != 0;
+}
+bool on16(const void *p, int64_t a, int64_t b, int es) { return reinterpret_cast<uintptr_t>(p) % 16 == 0 && a * es % 16 == 0 && b * es % 16 == 0; }
+
+struct Plan { nm::Layout l; int v, nv; size_t smem; bool wide; };
+constexpr int kSMs = 148;
+
+Plan plan(const Norm &P, int dt, bool bwd) {
+    Plan r{};
+    const int es = dt == CS2D_F32 ? 4 : 2, V = 16 / es;
+    const bool image = P.x_cs != 1;
+    bool vec = P.dim % V == 0 && on16(P.y, 0, 0, es) && (!P.gate || on16(P.gate, P.g_os, P.g_is, es)) && on16(P.weight, 0, 0, 1) && on16(P.bias, 0, 0, 1);
+    if (!image) vec = vec && on16(P.x, P.x_os, P.x_is, es);
+    if (bwd) vec = vec && on16(P.dy, P.dy_os, P.dy_is, es) && on16(P.dgate, 0, 0, es) && (image || on16(P.dx, P.dx_os, P.dx_is, es));
+    r.v = vec ? V : 1;
+    r.wide = !lanes_of(P.dim, r.v, dt, &r.l.T, &r.nv);
+    // images whose gradient is not one, and the other way round, take the wide kernels too
+    if (bwd && image != (P.dx_cs != 1)) r.wide = true;
+    if (image) {
+        const int64_t row = (int64_t)P.dim * es;
+        r.l.pitch = (int)(es == 2 ? (row + 63) / 128 * 128 + 64 : (row + 127) / 128 * 128 + 16);
+        r.l.P = 32;
+        while (r.l.P > 8 && r.l.P * (int64_t)r.l.pitch > 104 * 1024) r.l.P >>= 1;
+        if (r.l.P * (int64_t)r.l.pitch > 220 * 1024) r.wide = true;
+        r.l.whole = P.inner * es % 16 == 0 && on16(P.x, P.x_os, P.x_cs, es) && (!bwd || on16(P.dx, P.dx_os, P.dx_cs, es));
+        r.l.tiles = (P.inner + r.l.P - 1) / r.l.P;
+    }
+    if (r.wide) return r;
+    const int64_t tile = image ? r.l.P * (int64_t)r.l.pitch : 0, acc = bwd ? 8 * (int64_t)P.dim : 0;
+    r.smem = (size_t)(tile > acc ? tile : acc);
+    const int64_t work = image ? P.rows / P.inner * r.l.tiles : (P.rows + nm::NT / r.l.T - 1) / (nm::NT / r.l.T);
+    const int per = bwd ? 2 : 8;
+    r.l.grid = (int)(work < kSMs * per ? work : kSMs * per);
+    return r;
+}
+
+template <int DT> cudaError_t wide(const Norm &P, bool bwd, cudaStream_t st) {
+    const unsigned grid = (unsigned)((P.rows + NW - 1) / NW);
+    if (!bwd) {
+        wide_fwd<DT><<<grid, NW * 32, 0, st>>>(P);
+        return cudaGetLastError();
+    }
+    wide_bwd<DT><<<grid, NW * 32, 0, st>>>(P);
+    if (P.part) wide_part<DT><<<dim3((P.dim + NW * 32 - 1) / (NW * 32), P.parts), NW * 32, 0, st>>>(P);
     return cudaGetLastError();
+}
+cudaError_t wide(const Norm &P, int dt, bool bwd, cudaStream_t st) {
+    return dt == CS2D_F32 ? wide<CS2D_F32>(P, bwd, st) : dt == CS2D_F16 ? wide<CS2D_F16>(P, bwd, st) : wide<CS2D_BF16>(P, bwd, st);
 }
 
 }  // namespace
 
-int norm_parts(const Norm &P, int) { return (int)(P.rows < 512 ? (P.rows < 1 ? 1 : P.rows) : 512); }
+// Slots of the parameters' gradients: at most as many as CTAs of any of the kernels.
+int norm_parts(const Norm &P, int) { return (int)(P.rows < 2 * kSMs ? P.rows : 2 * kSMs); }
 
 cudaError_t launch_norm_fwd(const Norm &P, int dt, cudaStream_t st) {
-    const unsigned grid = (unsigned)((P.rows + NW - 1) / NW);
-    switch (dt) {
-        case CS2D_F32: norm_fwd<CS2D_F32><<<grid, NW * 32, 0, st>>>(P); break;
-        case CS2D_F16: norm_fwd<CS2D_F16><<<grid, NW * 32, 0, st>>>(P); break;
-        default: norm_fwd<CS2D_BF16><<<grid, NW * 32, 0, st>>>(P);
-    }
-    return cudaGetLastError();
+    const Plan r = plan(P, dt, false);
+    if (r.wide) return wide(P, dt, false, st);
+    return (dt == CS2D_F32 ? nm::fwd_f32 : dt == CS2D_F16 ? nm::fwd_f16 : nm::fwd_bf16)(P, r.l, r.v, r.nv, r.smem, st);
 }
-cudaError_t launch_norm_bwd(const Norm &P, int dt, cudaStream_t st) {
-    switch (dt) {
-        case CS2D_F32: return bwd<CS2D_F32>(P, st);
-        case CS2D_F16: return bwd<CS2D_F16>(P, st);
-        default: return bwd<CS2D_BF16>(P, st);
-    }
+cudaError_t launch_norm_bwd(const Norm &P_, int dt, cudaStream_t st, int *launches) {
+    Norm P = P_;
+    if (!P.dweight && !P.dbias) P.part = nullptr;
+    const Plan r = plan(P, dt, true);
+    if (!r.wide) P.parts = r.l.grid;
+    *launches = !P.part ? 1 : r.wide ? 3 : 2;
+    const cudaError_t e = r.wide ? wide(P, dt, true, st) : (dt == CS2D_F32 ? nm::bwd_f32 : dt == CS2D_F16 ? nm::bwd_f16 : nm::bwd_bf16)(P, r.l, r.v, r.nv, r.smem, st);
+    if (e != cudaSuccess || !P.part) return e;
+    norm_join<<<(2 * P.dim + 31) / 32, NW * 32, 0, st>>>(P);
+    return cudaGetLastError();
 }
 
 }  // namespace cs2d

@@ -1,0 +1,3 @@
+#include "cs2d_norm.cuh"
+
+namespace cs2d { namespace nm { cudaError_t fwd_f32(const Norm &P, const Layout &l, int v, int nv, size_t smem, cudaStream_t st) { return launch<false, CS2D_F32>(P, l, v, nv, smem, st); } } }

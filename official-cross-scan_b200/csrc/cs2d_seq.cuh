@@ -54,7 +54,7 @@ struct Norm {
 };
 int norm_parts(const Norm &P, int dt);
 cudaError_t launch_norm_fwd(const Norm &P, int dt, cudaStream_t st);
-cudaError_t launch_norm_bwd(const Norm &P, int dt, cudaStream_t st);
+cudaError_t launch_norm_bwd(const Norm &P, int dt, cudaStream_t st, int *launches);
 
 // ---- element types ---------------------------------------------------------------------------------------
 template <int DT> struct Elem;

@@ -146,7 +146,9 @@ int cs2d_norm_bwd(const cs2d_norm *p, const void *dy, int64_t dy_os, int64_t dy_
     Norm d = fill(p);
     d.dy = dy; d.dy_os = dy_os; d.dy_is = dy_is; d.stats = const_cast<float *>(stats); d.part = (float *)scratch;
     d.dx = dx; d.dx_os = dx_os; d.dx_is = dx_is; d.dx_cs = dx_cs; d.dgate = dgate; d.dweight = dweight; d.dbias = dbias;
-    return launched(launch_norm_bwd(d, p->io_dtype, static_cast<cudaStream_t>(stream)), dweight || dbias ? 3 : 1);
+    int n = 0;
+    const cudaError_t e = launch_norm_bwd(d, p->io_dtype, static_cast<cudaStream_t>(stream), &n);
+    return launched(e, n);
 }
 
 }  // extern "C"
