@@ -106,26 +106,30 @@ __device__ __forceinline__ void put(void *p, int dt, int i, float v) {
     else if (dt == CS2D_F16) ((__half *)p)[i] = __float2half_rn(v);
     else ((__nv_bfloat16 *)p)[i] = __float2bfloat16_rn(v);
 }
-// 32 channels of one sum, the parts in a fixed order
-__global__ void __launch_bounds__(NW * 32) norm_join(const Norm P) {
-    __shared__ float s[NW][32];
+// 32 channels of one sum, the parts in a fixed order: warp w adds parts w, w + 32, ...
+__global__ void __launch_bounds__(1024) norm_join(const Norm P) {
+    __shared__ float s[32][33];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, i = blockIdx.x * 32 + lane;
     float v = 0.f;
-    if (i < 2 * P.dim)
-        for (int k = warp; k < P.parts; k += NW) v += P.part[(int64_t)k * 2 * P.dim + i];
+    if (i < 2 * P.dim) {
+#pragma unroll 4
+        for (int k = warp; k < P.parts; k += 32) v += P.part[(int64_t)k * 2 * P.dim + i];
+    }
     s[warp][lane] = v;
     __syncthreads();
-    if (warp || i >= 2 * P.dim) return;
-    for (int k = 1; k < NW; ++k) v += s[k][lane];
-    if (i < P.dim) put(P.dweight, P.wtype, i, v);
-    else put(P.dbias, P.wtype, i - P.dim, v);
+    v = s[lane][warp];   // warp w: channel w of the block
+#pragma unroll
+    for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(~0u, v, o);
+    const int c = blockIdx.x * 32 + warp;
+    if (lane || c >= 2 * P.dim) return;
+    if (c < P.dim) put(P.dweight, P.wtype, c, v);
+    else put(P.dbias, P.wtype, c - P.dim, v);
 }
 
-
 // Lanes of a row and vectors of a lane: the fewest places for the row's vectors, of equal ones the fewest lanes (fewer shuffles).
-bool lanes_of(int dim, int v, int dt, int *T, int *nv) {
+bool lanes_of(int dim, int v, int dt, bool bwd, int *T, int *nv) {
     static const int narrow[] = {1, 2, 3, 0}, f32[] = {1, 2, 3, 6, 0}, single[] = {4, 12, 24, 0};
-    const int *set = v == 1 ? single : dt == CS2D_F32 ? f32 : narrow;
+    const int *set = v == 1 ? single : dt == CS2D_F32 && !bwd ? f32 : narrow;
     const int nvec = dim / v;
     int best = 0;
     for (int t = 1; t <= nm::NT; t <<= 1)
@@ -149,24 +153,28 @@ Plan plan(const Norm &P, int dt, bool bwd) {
     if (!image) vec = vec && on16(P.x, P.x_os, P.x_is, es);
     if (bwd) vec = vec && on16(P.dy, P.dy_os, P.dy_is, es) && on16(P.dgate, 0, 0, es) && (image || on16(P.dx, P.dx_os, P.dx_is, es));
     r.v = vec ? V : 1;
-    r.wide = !lanes_of(P.dim, r.v, dt, &r.l.T, &r.nv);
+    r.wide = !lanes_of(P.dim, r.v, dt, bwd, &r.l.T, &r.nv);
     // images whose gradient is not one, and the other way round, take the wide kernels too
     if (bwd && image != (P.dx_cs != 1)) r.wide = true;
+    if (r.wide) return r;
+    const int e = r.v * r.nv, per = bwd ? (e <= 8 ? 4 : e <= 12 && r.v > 1 ? 3 : 2) : 6, groups = nm::NT / r.l.T;
+    r.l.image = image;
     if (image) {
         const int64_t row = (int64_t)P.dim * es;
         r.l.pitch = (int)(es == 2 ? (row + 63) / 128 * 128 + 64 : (row + 127) / 128 * 128 + 16);
         r.l.P = 32;
-        while (r.l.P > 8 && r.l.P * (int64_t)r.l.pitch > 104 * 1024) r.l.P >>= 1;
-        if (r.l.P * (int64_t)r.l.pitch > 220 * 1024) r.wide = true;
+        while (r.l.P > 8 && r.l.P * (int64_t)r.l.pitch > (bwd ? 56 : 72) * 1024) r.l.P >>= 1;
+        if (r.l.P * (int64_t)r.l.pitch > (bwd ? 120 : 220) * 1024) r.wide = true;
         r.l.whole = P.inner * es % 16 == 0 && on16(P.x, P.x_os, P.x_cs, es) && (!bwd || on16(P.dx, P.dx_os, P.dx_cs, es));
-        r.l.tiles = (P.inner + r.l.P - 1) / r.l.P;
+        r.smem = (size_t)r.l.P * r.l.pitch;
+    } else {   // some rows per group and tile, as long as there are tiles for all CTAs
+        int k = 8;
+        while (k > 1 && P.rows < (int64_t)groups * k * kSMs * per) k >>= 1;
+        r.l.P = groups * k;
     }
-    if (r.wide) return r;
-    const int64_t tile = image ? r.l.P * (int64_t)r.l.pitch : 0, acc = bwd ? 8 * (int64_t)P.dim : 0;
-    r.smem = (size_t)(tile > acc ? tile : acc);
-    const int64_t work = image ? P.rows / P.inner * r.l.tiles : (P.rows + nm::NT / r.l.T - 1) / (nm::NT / r.l.T);
-    const int per = bwd ? 2 : 8;
-    r.l.grid = (int)(work < kSMs * per ? work : kSMs * per);
+    r.l.tiles = (P.inner + r.l.P - 1) / r.l.P;
+    r.l.tiles_all = P.rows / P.inner * r.l.tiles;
+    r.l.grid = (int)(r.l.tiles_all < kSMs * per ? r.l.tiles_all : kSMs * per);
     return r;
 }
 
@@ -187,7 +195,7 @@ cudaError_t wide(const Norm &P, int dt, bool bwd, cudaStream_t st) {
 }  // namespace
 
 // Slots of the parameters' gradients: at most as many as CTAs of any of the kernels.
-int norm_parts(const Norm &P, int) { return (int)(P.rows < 2 * kSMs ? P.rows : 2 * kSMs); }
+int norm_parts(const Norm &P, int) { return (int)(P.rows < 4 * kSMs ? P.rows : 4 * kSMs); }
 
 cudaError_t launch_norm_fwd(const Norm &P, int dt, cudaStream_t st) {
     const Plan r = plan(P, dt, false);
@@ -202,7 +210,7 @@ cudaError_t launch_norm_bwd(const Norm &P_, int dt, cudaStream_t st, int *launch
     *launches = !P.part ? 1 : r.wide ? 3 : 2;
     const cudaError_t e = r.wide ? wide(P, dt, true, st) : (dt == CS2D_F32 ? nm::bwd_f32 : dt == CS2D_F16 ? nm::bwd_f16 : nm::bwd_bf16)(P, r.l, r.v, r.nv, r.smem, st);
     if (e != cudaSuccess || !P.part) return e;
-    norm_join<<<(2 * P.dim + 31) / 32, NW * 32, 0, st>>>(P);
+    norm_join<<<(2 * P.dim + 31) / 32, 1024, 0, st>>>(P);
     return cudaGetLastError();
 }
 

@@ -21,12 +21,12 @@ namespace nm {
 
 constexpr int NT = 256;       // threads of a CTA
 constexpr int NWARP = NT / 32;
-constexpr int MAXE = 24;      // channels of a lane
+constexpr int MAXE = 24;      // channels of a lane, at most
 
 struct Layout {
-    int T, P, pitch;          // lanes of a row; positions of a tile and bytes between its rows in shared memory (images)
-    bool whole;               // tiles are read in 16-byte chunks
-    int64_t tiles;            // per outer index
+    int T, P, pitch;             // lanes of a row; rows of a tile; images: bytes between them in shared memory
+    bool image, whole;           // whole: tiles are read in 16-byte chunks
+    int64_t tiles, tiles_all;    // of an outer index; in all
     int grid;
 };
 
@@ -35,30 +35,112 @@ __device__ __forceinline__ float param(const void *p, int dt, int i, float none)
     return dt == CS2D_F32 ? ((const float *)p)[i] : dt == CS2D_F16 ? __half2float(((const __half *)p)[i]) : __bfloat162float(((const __nv_bfloat16 *)p)[i]);
 }
 
-// V consecutive parameters from channel d
-template <int V> __device__ __forceinline__ void params(float (&v)[V], const void *p, int dt, int d, float none) {
-    if (V > 1 && p && dt == CS2D_F32) {
-#pragma unroll
-        for (int k = 0; k < V; k += 4) {
-            const float4 t = *(const float4 *)((const float *)p + d + k);
-            v[k] = t.x; v[k + 1] = t.y; v[k + 2] = t.z; v[k + 3] = t.w;
-        }
-    } else {
-#pragma unroll
-        for (int k = 0; k < V; ++k) v[k] = param(p, dt, d + k, none);
-    }
+// Pairs of fp32 values, which one packed instruction serves
+__device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) { return __ffma2_rn(a, b, c); }
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) { return __fmul2_rn(a, b); }
+__device__ __forceinline__ float2 add2(float2 a, float2 b) { return __fadd2_rn(a, b); }
+template <int DT> __device__ __forceinline__ float2 pair_up(unsigned w) {
+    if constexpr (DT == CS2D_BF16) return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+    __half2 h;
+    memcpy(&h, &w, 4);
+    return __half22float2(h);
 }
+template <int DT> __device__ __forceinline__ unsigned pair_down(float2 v) {
+    unsigned w;
+    if constexpr (DT == CS2D_BF16) {
+        const __nv_bfloat162 t = __float22bfloat162_rn(v);
+        memcpy(&w, &t, 4);
+    } else {
+        const __half2 t = __float22half2_rn(v);
+        memcpy(&w, &t, 4);
+    }
+    return w;
+}
+
+// A lane's channels of a row: NV vectors of V elements, vector j of lane l being number j T + l of the row; H pairs of values.
+template <int DT, int V, int NV> struct Row {
+    using T = typename Elem<DT>::T;
+    using W = typename WordOf<sizeof(T) * V>::W;
+    static constexpr int H = NV * V / 2;
+    static __device__ __forceinline__ void up(const W (&w)[NV], float2 (&v)[H]) {
+        if constexpr (V == 1) {
+#pragma unroll
+            for (int h = 0; h < H; ++h) {
+                T a, b;
+                memcpy(&a, &w[2 * h], sizeof(T));
+                memcpy(&b, &w[2 * h + 1], sizeof(T));
+                v[h] = make_float2(Elem<DT>::up(a), Elem<DT>::up(b));
+            }
+        } else if constexpr (DT == CS2D_F32) {
+#pragma unroll
+            for (int j = 0; j < NV; ++j) memcpy(&v[j * 2], &w[j], 16);
+        } else {
+#pragma unroll
+            for (int j = 0; j < NV; ++j) {
+                unsigned t[4];
+                memcpy(t, &w[j], 16);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) v[j * 4 + k] = pair_up<DT>(t[k]);
+            }
+        }
+    }
+    // vector j of the values
+    static __device__ __forceinline__ W down(const float2 (&v)[H], int j) {
+        W w;
+        if constexpr (V == 1) {
+            const T t = Elem<DT>::down(j & 1 ? v[j / 2].y : v[j / 2].x);
+            memcpy(&w, &t, sizeof(T));
+        } else if constexpr (DT == CS2D_F32) {
+            memcpy(&w, &v[j * 2], 16);
+        } else {
+            unsigned t[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) t[k] = pair_down<DT>(v[j * 4 + k]);
+            memcpy(&w, t, 16);
+        }
+        return w;
+    }
+    static __device__ __forceinline__ void load(W (&w)[NV], const T *row, int l, int TL, int nvec, bool on) {
+#pragma unroll
+        for (int j = 0; j < NV; ++j) w[j] = on && j * TL + l < nvec ? *(const W *)(row + (j * TL + l) * V) : W{};
+    }
+    // weight or bias
+    static __device__ __forceinline__ void params(float2 (&v)[H], const void *p, int dt, int l, int TL, int nvec, float none) {
+        if (!p) {
+#pragma unroll
+            for (int h = 0; h < H; ++h) v[h] = both(none);
+        } else if (dt == CS2D_F32) {
+            constexpr int F = V < 4 ? 1 : 4;   // floats of an access
+            float t[NV * V];
+#pragma unroll
+            for (int j = 0; j < NV; ++j)
+#pragma unroll
+                for (int k = 0; k < V; k += F) {
+                    using G = typename WordOf<4 * F>::W;
+                    const G g = j * TL + l < nvec ? *(const G *)((const float *)p + (j * TL + l) * V + k) : G{};
+                    memcpy(&t[j * V + k], &g, sizeof(g));
+                }
+#pragma unroll
+            for (int h = 0; h < H; ++h) v[h] = make_float2(t[2 * h], t[2 * h + 1]);
+        } else {
+            W w[NV];
+            load(w, (const T *)p, l, TL, nvec, true);
+            up(w, v);
+        }
+    }
+};
 
 // Sums of two values over the T lanes of a row.  More than a warp: through shared memory, a named barrier per row group; two sets of
 // slots, so that the next sum may begin while others still read.
 struct Reduce {
     float2 (*slots)[NWARP];
     int T, parity;
-    __device__ __forceinline__ float2 operator()(float a, float b) {
+    template <bool TWO> __device__ __forceinline__ float2 of(float a, float b) {
         const int in_warp = T < 32 ? T : 32;
         for (int o = in_warp >> 1; o; o >>= 1) {
             a += __shfl_xor_sync(~0u, a, o);
-            b += __shfl_xor_sync(~0u, b, o);
+            if (TWO) b += __shfl_xor_sync(~0u, b, o);
         }
         if (T <= 32) return make_float2(a, b);
         const int warp = threadIdx.x >> 5, R = T / 32, first = warp / R * R;
@@ -67,7 +149,7 @@ struct Reduce {
         float2 s = slots[parity][first];
         for (int k = 1; k < R; ++k) {
             s.x += slots[parity][first + k].x;
-            s.y += slots[parity][first + k].y;
+            if (TWO) s.y += slots[parity][first + k].y;
         }
         parity ^= 1;
         return s;
@@ -140,211 +222,283 @@ template <int DT, bool IN> __device__ __forceinline__ void move_tile(unsigned ch
     }
 }
 
-// ---- rows ------------------------------------------------------------------------------------------------------
-// A lane's channels of a row: NV vectors of V, vector j of lane l being number j T + l of the row.
-template <int DT, int V, int NV> struct Row {
-    using P = Pack<DT, V>;
-    using W = typename P::W;
-    static __device__ __forceinline__ void load(W (&w)[NV], const typename Elem<DT>::T *row, int l, int T, int nvec, bool on) {
-#pragma unroll
-        for (int j = 0; j < NV; ++j) w[j] = on && j * T + l < nvec ? *(const W *)(row + (int64_t)(j * T + l) * V) : W{};
+// ---- kernels ---------------------------------------------------------------------------------------------------
+// CTAs go through tiles of P rows of an outer index.
+struct Tile {
+    int64_t o, i, row;   // outer index, first row of it, first row of all
+    int n;               // rows that are there
+    __device__ __forceinline__ Tile(const Norm &P, const Layout &l, int64_t t) {
+        o = l.tiles_all == l.tiles ? 0 : (unsigned)t / (unsigned)l.tiles;
+        i = (t - o * l.tiles) * l.P;
+        row = o * P.inner + i;
+        n = (int)min((int64_t)l.P, P.inner - i);
     }
 };
 
+// CTAs that an SM is to hold: the lane's values, a parameter's and the gate's, and 25 registers more
+template <int DT, int V, int NV, bool GATED> constexpr int FWD_CTAS = NV * V <= 8 ? 6 : NV * V < 16 ? 4 : GATED && (DT == CS2D_F32 || V == 1) ? 2 : 3;
+
 template <int DT, int V, int NV, bool GATED, bool IMAGE>
-__global__ void __launch_bounds__(NT, 2) norm_fwd(const Norm P, const Layout lay) {
+__global__ void __launch_bounds__(NT, (FWD_CTAS<DT, V, NV, GATED>)) norm_fwd(const Norm P, const Layout lay) {
     using R = Row<DT, V, NV>;
     using W = typename R::W;
-    using T = typename Elem<DT>::T;
+    using T = typename R::T;
     constexpr bool FULL = DT == CS2D_F32;
+    constexpr int H = R::H;
     extern __shared__ __align__(16) unsigned char tile[];
     __shared__ float2 slots[2][NWARP];
     Reduce sum{slots, lay.T, 0};
     const int TL = lay.T, l = threadIdx.x % TL, g = threadIdx.x / TL, groups = NT / TL, nvec = P.dim / V;
     const float inv = 1.f / P.dim;
-    auto work = [&](int64_t row, const T *x, int p, bool on) {
-        W xw[NV], zw[GATED ? NV : 1];
-        const int64_t o = on ? row / P.inner : 0, i = on ? row % P.inner : 0;
+    const int64_t x_step = groups * P.x_is, z_step = groups * P.g_is;
+    for (int64_t t = blockIdx.x; t < lay.tiles_all; t += gridDim.x) {
+        const Tile tl(P, lay, t);
         if constexpr (IMAGE) {
+            move_tile<DT, true>(tile, lay, (T *)P.x + tl.o * P.x_os + tl.i, P.x_cs, P.dim, tl.n);
+            __syncthreads();
+        }
+        const T *xp = (const T *)P.x + tl.o * P.x_os + (tl.i + g) * P.x_is, *zp = (const T *)P.gate + tl.o * P.g_os + (tl.i + g) * P.g_is;
+        for (int p0 = 0; p0 < tl.n; p0 += groups) {
+            const int p = p0 + g;
+            const bool on = p < tl.n;
+            W xw[NV], zw[GATED ? NV : 1];
+            if constexpr (IMAGE) {
+#pragma unroll
+                for (int j = 0; j < NV; ++j)
+                    xw[j] = on && j * TL + l < nvec ? *(const W *)element<sizeof(T)>(tile, lay.pitch, p, (j * TL + l) * V) : W{};
+            } else {
+                R::load(xw, xp, l, TL, nvec, on);
+                xp += x_step;
+            }
+            if constexpr (GATED) {
+                R::load(zw, zp, l, TL, nvec, on);
+                zp += z_step;
+            }
+            float2 x[H], s = both(0.f);
+            R::up(xw, x);
+#pragma unroll
+            for (int h = 0; h < H; ++h) s = add2(s, x[h]);
+            const float mean = sum.of<false>(s.x + s.y, 0.f).x * inv;
+            s = both(0.f);
+#pragma unroll
+            for (int j = 0; j < NV; ++j) {   // what lies behind the last channel stays out of the variance
+                const bool here = j * TL + l < nvec;
+                if constexpr (V == 1) {
+                    float &v = j & 1 ? x[j / 2].y : x[j / 2].x;
+                    v = here ? v - mean : 0.f;
+                    s.x = fmaf(v, v, s.x);
+                } else {
+#pragma unroll
+                    for (int k = 0; k < V / 2; ++k) {
+                        float2 &v = x[j * V / 2 + k];
+                        v = add2(v, both(-mean));
+                        if (here) s = fma2(v, v, s);
+                    }
+                }
+            }
+            const float rstd = rsqrtf(sum.of<false>(s.x + s.y, 0.f).x * inv + P.eps);
+            if (!on) continue;
+            if (P.stats && l == 0) ((float2 *)P.stats)[tl.row + p] = make_float2(mean, rstd);
+            float2 w[H];
+            R::params(w, P.weight, P.wtype, l, TL, nvec, 1.f);
+#pragma unroll
+            for (int h = 0; h < H; ++h) x[h] = mul2(x[h], mul2(w[h], both(rstd)));
+            R::params(w, P.bias, P.wtype, l, TL, nvec, 0.f);
+#pragma unroll
+            for (int h = 0; h < H; ++h) x[h] = add2(x[h], w[h]);
+            if constexpr (GATED) {
+                R::up(zw, w);
+#pragma unroll
+                for (int h = 0; h < H; ++h) x[h] = mul2(x[h], mul2(w[h], make_float2(sigmoid<FULL>(w[h].x), sigmoid<FULL>(w[h].y))));
+            }
+            T *y = (T *)P.y + (tl.row + p) * P.dim;
 #pragma unroll
             for (int j = 0; j < NV; ++j)
-                xw[j] = on && j * TL + l < nvec ? *(const W *)element<sizeof(T)>(tile, lay.pitch, p, (j * TL + l) * V) : W{};
-        } else {
-            R::load(xw, x + o * P.x_os + i * P.x_is, l, TL, nvec, on);
+                if (j * TL + l < nvec) *(W *)(y + (j * TL + l) * V) = R::down(x, j);
         }
-        if constexpr (GATED) R::load(zw, (const T *)P.gate + o * P.g_os + i * P.g_is, l, TL, nvec, on);
-        float s = 0.f, q = 0.f;
-#pragma unroll
-        for (int j = 0; j < NV; ++j) {
-            float v[V];
-            R::P::up(xw[j], v);
-#pragma unroll
-            for (int k = 0; k < V; ++k) s += v[k];
-        }
-        const float mean = sum(s, 0.f).x * inv;
-#pragma unroll
-        for (int j = 0; j < NV; ++j) {
-            float v[V];
-            R::P::up(xw[j], v);
-#pragma unroll
-            for (int k = 0; k < V; ++k) {
-                const float m = j * TL + l < nvec ? v[k] - mean : 0.f;
-                q = fmaf(m, m, q);
-            }
-        }
-        const float rstd = rsqrtf(sum(q, 0.f).x * inv + P.eps);
-        if (!on) return;
-        if (P.stats && l == 0) ((float2 *)P.stats)[row] = make_float2(mean, rstd);
-        T *y = (T *)P.y + row * P.dim;
-#pragma unroll
-        for (int j = 0; j < NV; ++j) {
-            const int vec = j * TL + l;
-            if (vec >= nvec) continue;
-            float v[V], w[V], b[V], z[V];
-            R::P::up(xw[j], v);
-            params<V>(w, P.weight, P.wtype, vec * V, 1.f);
-            params<V>(b, P.bias, P.wtype, vec * V, 0.f);
-            if constexpr (GATED) R::P::up(zw[j], z);
-#pragma unroll
-            for (int k = 0; k < V; ++k) {
-                v[k] = fmaf((v[k] - mean) * rstd, w[k], b[k]);
-                if (GATED) v[k] *= z[k] * sigmoid<FULL>(z[k]);
-            }
-            *(W *)(y + (int64_t)vec * V) = R::P::down(v);
-        }
-    };
-    if constexpr (IMAGE) {
-        const int64_t all = P.rows / P.inner * lay.tiles;
-        for (int64_t t = blockIdx.x; t < all; t += gridDim.x) {
-            const int64_t o = t / lay.tiles, p0 = t % lay.tiles * lay.P;
-            const int n = (int)min((int64_t)lay.P, P.inner - p0);
-            move_tile<DT, true>(tile, lay, (T *)P.x + o * P.x_os + p0, P.x_cs, P.dim, n);
-            __syncthreads();
-            for (int p = g; p < (n + groups - 1) / groups * groups; p += groups) work(o * P.inner + p0 + p, nullptr, p, p < n);
-            __syncthreads();
-        }
-    } else {
-        for (int64_t r = (int64_t)blockIdx.x * groups; r < P.rows; r += (int64_t)gridDim.x * groups) work(r + g, (const T *)P.x, 0, r + g < P.rows);
+        if constexpr (IMAGE) __syncthreads();
     }
 }
 
+template <int DT, int V, int NV, bool GATED> constexpr int BWD_CTAS = NV * V <= 8 ? 4 : NV * V <= 12 && V > 1 ? 3 : 2;
+// Rows are copied to shared memory one row ahead: every lane copies the vectors that it will read itself, so nobody waits for others.
+template <int BYTES> __device__ __forceinline__ void copy_async(void *dst, const void *src) {
+    if constexpr (BYTES == 16)
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((unsigned)__cvta_generic_to_shared(dst)), "l"(src) : "memory");
+    else
+        asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"((unsigned)__cvta_generic_to_shared(dst)), "l"(src) : "memory");
+}
+template <int V, int NV, bool GATED, bool IMAGE> constexpr int STAGE_BYTES = V == 1 ? 0 : NT * (16 * NV * (1 + GATED + !IMAGE) + 8);   // one row ahead, per CTA
+
 template <int DT, int V, int NV, bool GATED, bool IMAGE>
-__global__ void __launch_bounds__(NT, 2) norm_bwd(const Norm P, const Layout lay) {
+__global__ void __launch_bounds__(NT, (BWD_CTAS<DT, V, NV, GATED>)) norm_bwd(const Norm P, const Layout lay) {
     using R = Row<DT, V, NV>;
     using W = typename R::W;
-    using T = typename Elem<DT>::T;
-    constexpr bool FULL = DT == CS2D_F32;
-    extern __shared__ __align__(16) unsigned char tile[];
+    using T = typename R::T;
+    constexpr bool FULL = DT == CS2D_F32, AHEAD = V > 1;
+    constexpr int H = R::H, STAGE = STAGE_BYTES<V, NV, GATED, IMAGE>;
+    extern __shared__ __align__(16) unsigned char smem[];
+    unsigned char *tile = smem + 2 * STAGE;
     __shared__ float2 slots[2][NWARP];
     Reduce sum{slots, lay.T, 0};
     const int TL = lay.T, l = threadIdx.x % TL, g = threadIdx.x / TL, groups = NT / TL, nvec = P.dim / V;
     const float inv = 1.f / P.dim;
-    float dw[NV][V], db[NV][V];
-#pragma unroll
-    for (int j = 0; j < NV; ++j)
-#pragma unroll
-        for (int k = 0; k < V; ++k) dw[j][k] = db[j][k] = 0.f;
-    auto work = [&](int64_t row, int p, bool on) {
-        W xw[NV], dw_[NV], zw[GATED ? NV : 1];
-        const int64_t o = on ? row / P.inner : 0, i = on ? row % P.inner : 0;
-        if constexpr (IMAGE) {
-#pragma unroll
-            for (int j = 0; j < NV; ++j)
-                xw[j] = on && j * TL + l < nvec ? *(const W *)element<sizeof(T)>(tile, lay.pitch, p, (j * TL + l) * V) : W{};
-        } else {
-            R::load(xw, (const T *)P.x + o * P.x_os + i * P.x_is, l, TL, nvec, on);
-        }
-        R::load(dw_, (const T *)P.dy + o * P.dy_os + i * P.dy_is, l, TL, nvec, on);
-        if constexpr (GATED) R::load(zw, (const T *)P.gate + o * P.g_os + i * P.g_is, l, TL, nvec, on);
-        const float2 st = on ? ((const float2 *)P.stats)[row] : make_float2(0.f, 0.f);
-        float xh[NV][V], t[NV][V], s1 = 0.f, s2 = 0.f;
-#pragma unroll
-        for (int j = 0; j < NV; ++j) {
-            const int vec = j * TL + l;
-            const bool here = on && vec < nvec;
-            float w[V], b[V], z[V], dz[V];
-            R::P::up(xw[j], xh[j]);
-            R::P::up(dw_[j], t[j]);
-            if constexpr (GATED) R::P::up(zw[j], z);
-            params<V>(w, here ? P.weight : nullptr, P.wtype, vec * V, 1.f);
-            if constexpr (GATED) params<V>(b, here ? P.bias : nullptr, P.wtype, vec * V, 0.f);
-#pragma unroll
-            for (int k = 0; k < V; ++k) {
-                const float h = here ? (xh[j][k] - st.x) * st.y : 0.f;
-                float d = t[j][k];
-                if constexpr (GATED) {
-                    const float sg = sigmoid<FULL>(z[k]), silu = z[k] * sg, n = fmaf(h, w[k], b[k]);
-                    dz[k] = d * n * fmaf(silu, 1.f - sg, sg);
-                    d *= silu;
-                }
-                db[j][k] += d;
-                dw[j][k] = fmaf(d, h, dw[j][k]);
-                d *= w[k];
-                s1 += d;
-                s2 = fmaf(d, h, s2);
-                xh[j][k] = h;
-                t[j][k] = d;
-            }
-            if constexpr (GATED)
-                if (here) *(W *)((T *)P.dgate + row * P.dim + (int64_t)vec * V) = R::P::down(dz);
-        }
-        const float2 s = sum(s1, s2);
-        s1 = s.x * inv;
-        s2 = s.y * inv;
-        if (!on) return;
-        T *dx = (T *)P.dx + o * P.dx_os + i * P.dx_is;
-#pragma unroll
-        for (int j = 0; j < NV; ++j) {
-            const int vec = j * TL + l;
-            if (vec >= nvec) continue;
-            float v[V];
-#pragma unroll
-            for (int k = 0; k < V; ++k) v[k] = st.y * (t[j][k] - s1 - xh[j][k] * s2);
-            if constexpr (IMAGE) *(W *)element<sizeof(T)>(tile, lay.pitch, p, vec * V) = R::P::down(v);
-            else *(W *)(dx + (int64_t)vec * V) = R::P::down(v);
-        }
+    const int64_t x_step = groups * P.x_is, z_step = groups * P.g_is, d_step = groups * P.dy_is;
+    // the lane's vectors in a stage: stats, dy, z, x
+    auto vec_at = [&](int stage, int k, int j) { return (W *)(smem + stage * STAGE + NT * 8 + ((k * NV + j) * NT + threadIdx.x) * 16); };
+    auto stat_at = [&](int stage) { return (float2 *)(smem + stage * STAGE + threadIdx.x * 8); };
+    // the row that is copied next
+    const T *xp = nullptr, *dp = nullptr, *zp = nullptr;
+    const float2 *sp = nullptr;
+    int p_next = 0, n_next = 0;
+    int64_t t_next = blockIdx.x;
+    auto enter = [&]() {   // the first row of tile t_next
+        p_next = n_next = 0;
+        if (t_next >= lay.tiles_all) return;
+        const Tile tl(P, lay, t_next);
+        n_next = tl.n;
+        xp = (const T *)P.x + tl.o * P.x_os + (tl.i + g) * P.x_is + l * V;
+        dp = (const T *)P.dy + tl.o * P.dy_os + (tl.i + g) * P.dy_is + l * V;
+        zp = (const T *)P.gate + tl.o * P.g_os + (tl.i + g) * P.g_is + l * V;
+        sp = (const float2 *)P.stats + tl.row + g;
+        t_next += gridDim.x;
     };
-    if constexpr (IMAGE) {
-        const int64_t all = P.rows / P.inner * lay.tiles;
-        for (int64_t t = blockIdx.x; t < all; t += gridDim.x) {
-            const int64_t o = t / lay.tiles, p0 = t % lay.tiles * lay.P;
-            const int n = (int)min((int64_t)lay.P, P.inner - p0);
-            move_tile<DT, true>(tile, lay, (T *)P.x + o * P.x_os + p0, P.x_cs, P.dim, n);
-            __syncthreads();
-            for (int p = g; p < (n + groups - 1) / groups * groups; p += groups) work(o * P.inner + p0 + p, p, p < n);
-            __syncthreads();
-            move_tile<DT, false>(tile, lay, (T *)P.dx + o * P.dx_os + p0, P.dx_cs, P.dim, n);
+    auto ahead = [&](int stage) {
+        if (p_next + g < n_next) {
+            copy_async<8>(stat_at(stage), sp);
+#pragma unroll
+            for (int j = 0; j < NV; ++j) {
+                if (j * TL + l >= nvec) continue;
+                copy_async<16>(vec_at(stage, 0, j), dp + j * TL * V);
+                if (GATED) copy_async<16>(vec_at(stage, 1, j), zp + j * TL * V);
+                if (!IMAGE) copy_async<16>(vec_at(stage, 1 + GATED, j), xp + j * TL * V);
+            }
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+        p_next += groups;
+        sp += groups;
+        dp += d_step;
+        if (GATED) zp += z_step;
+        if (!IMAGE) xp += x_step;
+        if (p_next >= n_next) enter();
+    };
+    float2 dw[H], db[H];
+#pragma unroll
+    for (int h = 0; h < H; ++h) dw[h] = db[h] = both(0.f);
+    int stage = 0;
+    if (AHEAD) {
+        enter();
+        ahead(0);
+    }
+    for (int64_t t = blockIdx.x; t < lay.tiles_all; t += gridDim.x) {
+        const Tile tl(P, lay, t);
+        if constexpr (IMAGE) {
+            move_tile<DT, true>(tile, lay, (T *)P.x + tl.o * P.x_os + tl.i, P.x_cs, P.dim, tl.n);
             __syncthreads();
         }
-    } else {
-        for (int64_t r = (int64_t)blockIdx.x * groups; r < P.rows; r += (int64_t)gridDim.x * groups) work(r + g, 0, r + g < P.rows);
+        T *zo = (T *)P.dgate + (tl.row + g) * P.dim + l * V, *xo = (T *)P.dx + tl.o * P.dx_os + (tl.i + g) * P.dx_is + l * V;
+        for (int p0 = 0; p0 < tl.n; p0 += groups, zo += groups * (int64_t)P.dim, xo += groups * P.dx_is) {
+            const int p = p0 + g;
+            const bool on = p < tl.n;
+            if (AHEAD) {
+                ahead(stage ^ 1);
+                asm volatile("cp.async.wait_group 1;" ::: "memory");
+            }
+            auto fetch = [&](W (&w)[NV], int k, const T *row) {
+                if constexpr (AHEAD) {
+#pragma unroll
+                    for (int j = 0; j < NV; ++j) w[j] = on && j * TL + l < nvec ? *vec_at(stage, k, j) : W{};
+                } else {
+                    R::load(w, row, l, TL, nvec, on);
+                }
+            };
+            W xw[NV], ww[NV];
+            if constexpr (IMAGE) {
+#pragma unroll
+                for (int j = 0; j < NV; ++j)
+                    xw[j] = on && j * TL + l < nvec ? *(const W *)element<sizeof(T)>(tile, lay.pitch, p, (j * TL + l) * V) : W{};
+            } else {
+                fetch(xw, 1 + GATED, (const T *)P.x + tl.o * P.x_os + (tl.i + p) * P.x_is);
+            }
+            const float2 st = !on ? both(0.f) : AHEAD ? *stat_at(stage) : ((const float2 *)P.stats)[tl.row + p];
+            float2 h[H], d[H], w[H];
+            R::up(xw, h);
+#pragma unroll
+            for (int k = 0; k < H; ++k) h[k] = mul2(add2(h[k], both(-st.x)), both(st.y));
+            fetch(ww, 0, (const T *)P.dy + tl.o * P.dy_os + (tl.i + p) * P.dy_is);
+            R::up(ww, d);
+            R::params(w, P.weight, P.wtype, l, TL, nvec, 1.f);
+            if constexpr (GATED) {
+                float2 z[H], b[H];
+                fetch(ww, 1, (const T *)P.gate + tl.o * P.g_os + (tl.i + p) * P.g_is);
+                R::up(ww, z);
+                R::params(b, P.bias, P.wtype, l, TL, nvec, 0.f);
+#pragma unroll
+                for (int k = 0; k < H; ++k) {
+                    const float2 sg = make_float2(sigmoid<FULL>(z[k].x), sigmoid<FULL>(z[k].y)), silu = mul2(z[k], sg);
+                    const float2 slope = fma2(silu, add2(both(1.f), make_float2(-sg.x, -sg.y)), sg);
+                    z[k] = mul2(mul2(d[k], fma2(h[k], w[k], b[k])), slope);
+                    d[k] = mul2(d[k], silu);
+                }
+                if (on) {
+#pragma unroll
+                    for (int j = 0; j < NV; ++j)
+                        if (j * TL + l < nvec) *(W *)(zo + j * TL * V) = R::down(z, j);
+                }
+            }
+            // (rows and channels that are not there have dy = 0)
+            float2 s1 = both(0.f), s2 = both(0.f);
+#pragma unroll
+            for (int k = 0; k < H; ++k) {
+                db[k] = add2(db[k], d[k]);
+                dw[k] = fma2(d[k], h[k], dw[k]);
+                d[k] = mul2(d[k], w[k]);
+                s1 = add2(s1, d[k]);
+                s2 = fma2(d[k], h[k], s2);
+            }
+            const float2 s = sum.of<true>(s1.x + s1.y, s2.x + s2.y);
+            stage ^= 1;
+            if (!on) continue;
+            const float2 rs = both(st.y), c1 = both(-st.y * s.x * inv), c2 = both(-st.y * s.y * inv);
+#pragma unroll
+            for (int k = 0; k < H; ++k) d[k] = fma2(h[k], c2, fma2(d[k], rs, c1));
+#pragma unroll
+            for (int j = 0; j < NV; ++j) {
+                const int vec = j * TL + l;
+                if (vec >= nvec) continue;
+                if constexpr (IMAGE) *(W *)element<sizeof(T)>(tile, lay.pitch, p, vec * V) = R::down(d, j);
+                else *(W *)(xo + j * TL * V) = R::down(d, j);
+            }
+        }
+        if constexpr (IMAGE) {
+            __syncthreads();
+            move_tile<DT, false>(tile, lay, (T *)P.dx + tl.o * P.dx_os + tl.i, P.dx_cs, P.dim, tl.n);
+            __syncthreads();
+        }
     }
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
     if (!P.part) return;
     // the CTA's sums: over the rows of a warp by shuffles, over the groups one after the other
     for (int off = TL; off < 32; off <<= 1) {
 #pragma unroll
-        for (int j = 0; j < NV; ++j)
-#pragma unroll
-            for (int k = 0; k < V; ++k) {
-                dw[j][k] += __shfl_xor_sync(~0u, dw[j][k], off);
-                db[j][k] += __shfl_xor_sync(~0u, db[j][k], off);
-            }
+        for (int h = 0; h < H; ++h) {
+            dw[h] = add2(dw[h], make_float2(__shfl_xor_sync(~0u, dw[h].x, off), __shfl_xor_sync(~0u, dw[h].y, off)));
+            db[h] = add2(db[h], make_float2(__shfl_xor_sync(~0u, db[h].x, off), __shfl_xor_sync(~0u, db[h].y, off)));
+        }
     }
     const int per = TL < 32 ? 32 : TL, turns = NT / per;   // threads of a turn
-    float *acc = (float *)tile;
+    float *acc = (float *)smem;
     for (int turn = 0; turn < turns; ++turn) {
         __syncthreads();
         if ((int)threadIdx.x / per != turn || (int)threadIdx.x % per >= TL) continue;
 #pragma unroll
-        for (int j = 0; j < NV; ++j) {
-            const int vec = j * TL + l;
+        for (int e = 0; e < NV * V; ++e) {
+            const int vec = e / V * TL + l;
             if (vec >= nvec) continue;
-#pragma unroll
-            for (int k = 0; k < V; ++k) {
-                float *aw = acc + vec * V + k, *ab = aw + P.dim;
-                *aw = turn ? *aw + dw[j][k] : dw[j][k];
-                *ab = turn ? *ab + db[j][k] : db[j][k];
-            }
+            float *aw = acc + vec * V + e % V, *ab = aw + P.dim;
+            const float vw = e & 1 ? dw[e / 2].y : dw[e / 2].x, vb = e & 1 ? db[e / 2].y : db[e / 2].x;
+            *aw = turn ? *aw + vw : vw;
+            *ab = turn ? *ab + vb : vb;
         }
     }
     __syncthreads();
@@ -353,6 +507,8 @@ __global__ void __launch_bounds__(NT, 2) norm_bwd(const Norm P, const Layout lay
 
 // ---- launches ----------------------------------------------------------------------------------------------------
 template <class K> cudaError_t start(K *kernel, const Norm &P, const Layout &l, size_t smem, cudaStream_t st) {
+    const size_t acc = (size_t)8 * P.dim;   // the backward's sums, in the place of all else
+    if (P.dy && smem < acc) smem = acc;
     if (smem > 48 * 1024) {
         const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
         if (e != cudaSuccess) return e;
@@ -361,10 +517,12 @@ template <class K> cudaError_t start(K *kernel, const Norm &P, const Layout &l, 
     return cudaGetLastError();
 }
 template <bool BWD, int DT, int V, int NV> cudaError_t go(const Norm &P, const Layout &l, size_t smem, cudaStream_t st) {
-    const bool image = l.P > 0;
+    const bool image = l.image;
     if constexpr (BWD) {
-        if (P.gate) return image ? start(norm_bwd<DT, V, NV, true, true>, P, l, smem, st) : start(norm_bwd<DT, V, NV, true, false>, P, l, smem, st);
-        return image ? start(norm_bwd<DT, V, NV, false, true>, P, l, smem, st) : start(norm_bwd<DT, V, NV, false, false>, P, l, smem, st);
+        if (P.gate) return image ? start(norm_bwd<DT, V, NV, true, true>, P, l, smem + 2 * STAGE_BYTES<V, NV, true, true>, st)
+                                 : start(norm_bwd<DT, V, NV, true, false>, P, l, smem + 2 * STAGE_BYTES<V, NV, true, false>, st);
+        return image ? start(norm_bwd<DT, V, NV, false, true>, P, l, smem + 2 * STAGE_BYTES<V, NV, false, true>, st)
+                     : start(norm_bwd<DT, V, NV, false, false>, P, l, smem + 2 * STAGE_BYTES<V, NV, false, false>, st);
     } else {
         if (P.gate) return image ? start(norm_fwd<DT, V, NV, true, true>, P, l, smem, st) : start(norm_fwd<DT, V, NV, true, false>, P, l, smem, st);
         return image ? start(norm_fwd<DT, V, NV, false, true>, P, l, smem, st) : start(norm_fwd<DT, V, NV, false, false>, P, l, smem, st);
@@ -376,7 +534,7 @@ template <bool BWD, int DT> cudaError_t launch(const Norm &P, const Layout &l, i
             case 1: return go<BWD, DT, V, 1>(P, l, smem, st);
             case 2: return go<BWD, DT, V, 2>(P, l, smem, st);
             case 3: return go<BWD, DT, V, 3>(P, l, smem, st);
-            case 6: if constexpr (DT == CS2D_F32) return go<BWD, DT, V, 6>(P, l, smem, st);
+            case 6: if constexpr (DT == CS2D_F32 && !BWD) return go<BWD, DT, V, 6>(P, l, smem, st);
         }
     else switch (nv) {
             case 4: return go<BWD, DT, 1, 4>(P, l, smem, st);
