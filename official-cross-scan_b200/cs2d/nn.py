@@ -12,6 +12,7 @@ import torch
 from torch import nn
 
 from .cross import cross_scan_2d
+from .norm import layer_norm
 
 
 class CrossScan2D(nn.Module):
@@ -59,11 +60,15 @@ class SS2D(nn.Module):
     output, nothing is copied or transposed) -> dt_proj (per direction, rank -> d_inner; the
     softplus and ``dt_bias`` are applied inside the kernels) -> CrossScan2D (all directions and the
     fusion weights in one launch each way) -> LayerNorm -> gate with SiLU -> out_proj.
+
+    ``fused_norm``: the normalisation and the gate as one operator each way (``cs2d.layer_norm``), which reads the scan's
+    channel-major image as it lies and rounds once; same parameters and state dict.
     """
 
     def __init__(self, d_model: int, d_state: int = 16, expand: int = 2, dt_rank: int | None = None, d_conv: int = 3,
-                 directions: int = 4, device=None):
+                 directions: int = 4, device=None, fused_norm: bool = False):
         super().__init__()
+        self.fused_norm = fused_norm
         self.d_model, self.d_inner, self.d_state, self.K = d_model, expand * d_model, d_state, directions
         self.dt_rank = dt_rank or max(1, math.ceil(d_model / 16))
         d, R, N, K = self.d_inner, self.dt_rank, d_state, directions
@@ -89,5 +94,8 @@ class SS2D(nn.Module):
         delta = torch.einsum("bkrhw,kdr->bkdhw", dts, self.dt_proj.to(dts.dtype)).reshape(b, K * d, h, w)
         A = -torch.exp(self.scan.A_log.float())
         y = self._scan(u, delta, A, Bm, Cm, self.scan.fusion, self.scan.D, self.scan.dt_bias)
+        if self.fused_norm:
+            y = y.permute(0, 2, 3, 1).to(x.dtype)
+            return self.out_proj(layer_norm(y, self.out_norm.weight, self.out_norm.bias, z.to(x.dtype), self.out_norm.eps))
         y = self.out_norm(y.permute(0, 2, 3, 1).to(x.dtype))
         return self.out_proj(y * torch.nn.functional.silu(z))

@@ -112,7 +112,7 @@ __global__ void __launch_bounds__(1024) norm_join(const Norm P) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, i = blockIdx.x * 32 + lane;
     float v = 0.f;
     if (i < 2 * P.dim) {
-#pragma unroll 4
+#pragma unroll 8
         for (int k = warp; k < P.parts; k += 32) v += P.part[(int64_t)k * 2 * P.dim + i];
     }
     s[warp][lane] = v;
@@ -127,9 +127,9 @@ __global__ void __launch_bounds__(1024) norm_join(const Norm P) {
 }
 
 // Lanes of a row and vectors of a lane: the fewest places for the row's vectors, of equal ones the fewest lanes (fewer shuffles).
-bool lanes_of(int dim, int v, int dt, bool bwd, int *T, int *nv) {
-    static const int narrow[] = {1, 2, 3, 0}, f32[] = {1, 2, 3, 6, 0}, single[] = {4, 12, 24, 0};
-    const int *set = v == 1 ? single : dt == CS2D_F32 && !bwd ? f32 : narrow;
+bool lanes_of(int dim, int v, int dt, bool bwd, bool heavy, int *T, int *nv) {
+    static const int two[] = {1, 2, 0}, three[] = {1, 2, 3, 0}, f32[] = {1, 2, 3, 6, 0}, single[] = {4, 12, 24, 0};
+    const int *set = v == 1 ? single : bwd ? (heavy ? two : three) : dt == CS2D_F32 ? f32 : three;
     const int nvec = dim / v;
     int best = 0;
     for (int t = 1; t <= nm::NT; t <<= 1)
@@ -153,7 +153,7 @@ Plan plan(const Norm &P, int dt, bool bwd) {
     if (!image) vec = vec && on16(P.x, P.x_os, P.x_is, es);
     if (bwd) vec = vec && on16(P.dy, P.dy_os, P.dy_is, es) && on16(P.dgate, 0, 0, es) && (image || on16(P.dx, P.dx_os, P.dx_is, es));
     r.v = vec ? V : 1;
-    r.wide = !lanes_of(P.dim, r.v, dt, bwd, &r.l.T, &r.nv);
+    r.wide = !lanes_of(P.dim, r.v, dt, bwd, P.gate || image, &r.l.T, &r.nv);
     // images whose gradient is not one, and the other way round, take the wide kernels too
     if (bwd && image != (P.dx_cs != 1)) r.wide = true;
     if (r.wide) return r;
@@ -162,7 +162,8 @@ Plan plan(const Norm &P, int dt, bool bwd) {
     if (image) {
         const int64_t row = (int64_t)P.dim * es;
         r.l.pitch = (int)(es == 2 ? (row + 63) / 128 * 128 + 64 : (row + 127) / 128 * 128 + 16);
-        r.l.P = 32;
+        r.l.P = es == 2 ? 64 : 32;   // 128 bytes of a channel
+        while (r.l.P > 16 && (P.inner + r.l.P - 1) / r.l.P * (P.rows / P.inner) < 2 * kSMs) r.l.P >>= 1;
         while (r.l.P > 8 && r.l.P * (int64_t)r.l.pitch > (bwd ? 56 : 72) * 1024) r.l.P >>= 1;
         if (r.l.P * (int64_t)r.l.pitch > (bwd ? 120 : 220) * 1024) r.wide = true;
         r.l.whole = P.inner * es % 16 == 0 && on16(P.x, P.x_os, P.x_cs, es) && (!bwd || on16(P.dx, P.dx_os, P.dx_cs, es));

@@ -165,59 +165,86 @@ template <int ES> __device__ __forceinline__ unsigned char *element(unsigned cha
     return chunk<ES>(tile, pitch, p, d / (16 / ES)) + d % (16 / ES) * ES;
 }
 // IN: image -> tile, else tile -> image.  img: channel 0, first position; cs: elements between channels; n positions are there.
-template <int DT, bool IN> __device__ __forceinline__ void move_tile(unsigned char *tile, const Layout &l, typename Elem<DT>::T *img, int64_t cs, int dim, int n) {
+// U accesses at a time, reads before writes (two single elements count as one): the forward takes 6, the backward, whose sums are in registers
+// meanwhile, 4 on the way in and, where no latency is waited for, 1 on the way out (B16 D384 128x128 bf16: 328 us; 4 and 4: 400, 1 and 1: 387).
+template <int DT, bool IN, int U> __device__ __forceinline__ void move_tile(unsigned char *tile, const Layout &l, typename Elem<DT>::T *img, int64_t cs, int dim, int n) {
     using T = typename Elem<DT>::T;
     constexpr int ES = sizeof(T);
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    if (ES == 2 && l.whole && l.P == 32) {
+    if (ES == 2 && l.whole && l.P % 32 == 0) {
         // a warp takes 8 channels x 32 positions: lane t has 8 positions of channel t / 4.  Word k of the lanes is an 8 x 8 matrix whose column
         // c is position 8 (c / 2) + 2 k + c % 2; its transpose is eight 16-byte chunks, one per position.
-        const int m = lane >> 3, c = lane & 7, p = 8 * (c >> 1) + 2 * m + (c & 1), q = 8 * (lane & 3);
-#pragma unroll 4
-        for (int d0 = warp * 8; d0 < dim; d0 += NWARP * 8) {
-            const int d = d0 + (lane >> 2);
-            const bool ok = d < dim && q < n;
-            T *g = img + d * cs + q;
-            const unsigned s = (unsigned)__cvta_generic_to_shared(chunk<ES>(tile, l.pitch, p, d0 >> 3));
-            uint4 v = make_uint4(0, 0, 0, 0);
-            if constexpr (IN) {
-                if (ok) v = *(const uint4 *)g;
-                asm volatile("stmatrix.sync.aligned.m8n8.x4.trans.shared.b16 [%0], {%1, %2, %3, %4};" ::"r"(s), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
-            } else {
-                asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(s) : "memory");
-                if (ok) *(uint4 *)g = v;
+        const int m = lane >> 3, c = lane & 7, pm = 8 * (c >> 1) + 2 * m + (c & 1), qm = 8 * (lane & 3);
+        const int sh = l.P == 64, all = ((dim + 7) / 8) << sh;   // 128 bytes of a channel by two warps that follow each other
+        for (int w0 = warp; w0 < all; w0 += NWARP * U) {
+            uint4 v[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int w = w0 + u * NWARP, b32 = (w & sh) * 32, d = (w >> sh) * 8 + (lane >> 2);
+                const bool ok = w < all && d < dim && qm + b32 < n;
+                if (IN) v[u] = ok ? *(const uint4 *)(img + d * cs + qm + b32) : make_uint4(0, 0, 0, 0);
+                else if (w < all)
+                    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(v[u].x), "=r"(v[u].y), "=r"(v[u].z), "=r"(v[u].w)
+                                 : "r"((unsigned)__cvta_generic_to_shared(chunk<ES>(tile, l.pitch, pm + b32, w >> sh))) : "memory");
+            }
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int w = w0 + u * NWARP, b32 = (w & sh) * 32, d = (w >> sh) * 8 + (lane >> 2);
+                if (w >= all) continue;
+                if (IN)
+                    asm volatile("stmatrix.sync.aligned.m8n8.x4.trans.shared.b16 [%0], {%1, %2, %3, %4};" ::"r"(
+                                     (unsigned)__cvta_generic_to_shared(chunk<ES>(tile, l.pitch, pm + b32, w >> sh))),
+                                 "r"(v[u].x), "r"(v[u].y), "r"(v[u].z), "r"(v[u].w) : "memory");
+                else if (d < dim && qm + b32 < n) *(uint4 *)(img + d * cs + qm + b32) = v[u];
             }
         }
     } else if (ES == 4 && l.whole) {
-        const int per = l.P / 4;   // chunks of a channel
-#pragma unroll 4
-        for (int i = threadIdx.x; i < dim * per; i += NT) {
-            const int d = i / per, q = i % per * 4;
-            if (q >= n) continue;
-            T *g = img + d * cs + q;
-            if constexpr (IN) {
-                const float4 v = *(const float4 *)g;
-                *(float *)element<ES>(tile, l.pitch, q, d) = v.x;
-                *(float *)element<ES>(tile, l.pitch, q + 1, d) = v.y;
-                *(float *)element<ES>(tile, l.pitch, q + 2, d) = v.z;
-                *(float *)element<ES>(tile, l.pitch, q + 3, d) = v.w;
-            } else {
-                float4 v;
-                v.x = *(const float *)element<ES>(tile, l.pitch, q, d);
-                v.y = *(const float *)element<ES>(tile, l.pitch, q + 1, d);
-                v.z = *(const float *)element<ES>(tile, l.pitch, q + 2, d);
-                v.w = *(const float *)element<ES>(tile, l.pitch, q + 3, d);
-                *(float4 *)g = v;
+        const int sh = __ffs(l.P) - 3, all = dim << sh;   // chunks of a channel: P / 4
+        for (int i0 = threadIdx.x; i0 < all; i0 += NT * U) {
+            float4 v[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int i = i0 + u * NT, d = i >> sh, q = (i & ((1 << sh) - 1)) * 4;
+                const bool ok = i < all && q < n;
+                if (IN) v[u] = ok ? *(const float4 *)(img + d * cs + q) : make_float4(0.f, 0.f, 0.f, 0.f);
+                else if (ok) {
+                    v[u].x = *(const float *)element<ES>(tile, l.pitch, q, d);
+                    v[u].y = *(const float *)element<ES>(tile, l.pitch, q + 1, d);
+                    v[u].z = *(const float *)element<ES>(tile, l.pitch, q + 2, d);
+                    v[u].w = *(const float *)element<ES>(tile, l.pitch, q + 3, d);
+                }
+            }
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int i = i0 + u * NT, d = i >> sh, q = (i & ((1 << sh) - 1)) * 4;
+                if (i >= all || q >= n) continue;
+                if (IN) {
+                    *(float *)element<ES>(tile, l.pitch, q, d) = v[u].x;
+                    *(float *)element<ES>(tile, l.pitch, q + 1, d) = v[u].y;
+                    *(float *)element<ES>(tile, l.pitch, q + 2, d) = v[u].z;
+                    *(float *)element<ES>(tile, l.pitch, q + 3, d) = v[u].w;
+                } else {
+                    *(float4 *)(img + d * cs + q) = v[u];
+                }
             }
         }
     } else {
-#pragma unroll 8
-        for (int i = threadIdx.x; i < dim * l.P; i += NT) {
-            const int d = i / l.P, p = i % l.P;
-            if (p >= n) continue;
-            T *e = (T *)element<ES>(tile, l.pitch, p, d), *g = img + d * cs + p;
-            if constexpr (IN) *e = *g;
-            else *g = *e;
+        constexpr int N = 2 * U;
+        const int sh = __ffs(l.P) - 1, all = dim << sh;
+        for (int i0 = threadIdx.x; i0 < all; i0 += NT * N) {
+            T v[N];
+#pragma unroll
+            for (int u = 0; u < N; ++u) {
+                const int i = i0 + u * NT, d = i >> sh, p = i & (l.P - 1);
+                if (i < all && p < n) v[u] = IN ? img[d * cs + p] : *(const T *)element<ES>(tile, l.pitch, p, d);
+            }
+#pragma unroll
+            for (int u = 0; u < N; ++u) {
+                const int i = i0 + u * NT, d = i >> sh, p = i & (l.P - 1);
+                if (i >= all || p >= n) continue;
+                if (IN) *(T *)element<ES>(tile, l.pitch, p, d) = v[u];
+                else img[d * cs + p] = v[u];
+            }
         }
     }
 }
@@ -254,7 +281,7 @@ __global__ void __launch_bounds__(NT, (FWD_CTAS<DT, V, NV, GATED>)) norm_fwd(con
     for (int64_t t = blockIdx.x; t < lay.tiles_all; t += gridDim.x) {
         const Tile tl(P, lay, t);
         if constexpr (IMAGE) {
-            move_tile<DT, true>(tile, lay, (T *)P.x + tl.o * P.x_os + tl.i, P.x_cs, P.dim, tl.n);
+            move_tile<DT, true, 6>(tile, lay, (T *)P.x + tl.o * P.x_os + tl.i, P.x_cs, P.dim, tl.n);
             __syncthreads();
         }
         const T *xp = (const T *)P.x + tl.o * P.x_os + (tl.i + g) * P.x_is, *zp = (const T *)P.gate + tl.o * P.g_os + (tl.i + g) * P.g_is;
@@ -393,7 +420,7 @@ __global__ void __launch_bounds__(NT, (BWD_CTAS<DT, V, NV, GATED>)) norm_bwd(con
     for (int64_t t = blockIdx.x; t < lay.tiles_all; t += gridDim.x) {
         const Tile tl(P, lay, t);
         if constexpr (IMAGE) {
-            move_tile<DT, true>(tile, lay, (T *)P.x + tl.o * P.x_os + tl.i, P.x_cs, P.dim, tl.n);
+            move_tile<DT, true, 4>(tile, lay, (T *)P.x + tl.o * P.x_os + tl.i, P.x_cs, P.dim, tl.n);
             __syncthreads();
         }
         T *zo = (T *)P.dgate + (tl.row + g) * P.dim + l * V, *xo = (T *)P.dx + tl.o * P.dx_os + (tl.i + g) * P.dx_is + l * V;
@@ -472,7 +499,7 @@ __global__ void __launch_bounds__(NT, (BWD_CTAS<DT, V, NV, GATED>)) norm_bwd(con
         }
         if constexpr (IMAGE) {
             __syncthreads();
-            move_tile<DT, false>(tile, lay, (T *)P.dx + tl.o * P.dx_os + tl.i, P.dx_cs, P.dim, tl.n);
+            move_tile<DT, false, 1>(tile, lay, (T *)P.dx + tl.o * P.dx_os + tl.i, P.dx_cs, P.dim, tl.n);
             __syncthreads();
         }
     }
@@ -509,7 +536,7 @@ __global__ void __launch_bounds__(NT, (BWD_CTAS<DT, V, NV, GATED>)) norm_bwd(con
 template <class K> cudaError_t start(K *kernel, const Norm &P, const Layout &l, size_t smem, cudaStream_t st) {
     const size_t acc = (size_t)8 * P.dim;   // the backward's sums, in the place of all else
     if (P.dy && smem < acc) smem = acc;
-    if (smem > 48 * 1024) {
+    if (smem > 40 * 1024) {   // the default limit counts static shared memory too
         const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
         if (e != cudaSuccess) return e;
     }
@@ -533,7 +560,8 @@ template <bool BWD, int DT> cudaError_t launch(const Norm &P, const Layout &l, i
     if (v == V) switch (nv) {
             case 1: return go<BWD, DT, V, 1>(P, l, smem, st);
             case 2: return go<BWD, DT, V, 2>(P, l, smem, st);
-            case 3: return go<BWD, DT, V, 3>(P, l, smem, st);
+            case 3: if constexpr (BWD) return P.gate || l.image ? cudaErrorInvalidValue : start(norm_bwd<DT, V, 3, false, false>, P, l, smem + 2 * STAGE_BYTES<V, 3, false, false>, st);
+                    else return go<BWD, DT, V, 3>(P, l, smem, st);
             case 6: if constexpr (DT == CS2D_F32 && !BWD) return go<BWD, DT, V, 6>(P, l, smem, st);
         }
     else switch (nv) {

@@ -283,3 +283,32 @@ def test_scan_and_norm_as_a_block_runs_them():
     for name, a, b in zip(("x", *par), got, want):
         check_close("d" + name, a.cpu(), b, 1e-3, 1e-3)
     assert cs2d.device_status() == 0
+
+
+@pytest.mark.parametrize("dtype", (F32, BF16))
+def test_ss2d_with_the_fused_norm(dtype):
+    """The block with its norm and gate in one operator: the same step as with the three, to the roundings between them."""
+    import copy
+    from cs2d.nn import SS2D
+    torch.manual_seed(5)
+    m = SS2D(d_model=16, d_state=4).cuda()
+    f = SS2D(d_model=16, d_state=4, fused_norm=True).cuda()
+    f.load_state_dict(m.state_dict())
+    x = torch.randn(2, 8, 12, 16, device="cuda")
+    dy = torch.randn(2, 8, 12, 16, device="cuda")
+    if dtype == BF16:      # projections and norm in 16 bits, the scan's parameters in 32 as everywhere
+        for b in (m, f):
+            for p in (b.in_proj, b.conv2d, b.x_proj, b.out_norm, b.out_proj):
+                p.to(BF16)
+        x, dy = x.to(BF16), dy.to(BF16)
+    outs = []
+    for b in (m, f):
+        xl = x.clone().requires_grad_(True)
+        y = b(xl)
+        outs.append((y, *torch.autograd.grad(y, [xl, *b.parameters()], dy)))
+    # fp32: a block-level tolerance; bf16: the three operators round the norm and the gate's value on the way, half a step each
+    tol = 1e-4 if dtype == F32 else 12 * R.half_step(BF16)
+    for name, a, c in zip(("y", "x", *dict(m.named_parameters())), *outs):
+        scale = float(a.float().abs().max())
+        check_close(name, c.detach().float().cpu(), a.detach().float().cpu(), tol, tol * max(scale, 1e-3))
+    assert cs2d.device_status() == 0
