@@ -148,81 +148,93 @@ __device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_
 template <int LEFT> __device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(LEFT) : "memory"); }
 
 template <int BYTES> __device__ __forceinline__ void copy_async(void *dst, const void *src) {
-    static_assert(BYTES == 16, "the whole chunk");
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((unsigned)__cvta_generic_to_shared(dst)), "l"(src) : "memory");
+    const unsigned d = (unsigned)__cvta_generic_to_shared(dst);
+    if constexpr (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(d), "l"(src) : "memory");
+    else asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(d), "l"(src) : "memory");
 }
 
 // A tensor as a warp walks it: `at` is the address of the first channel of its unit in the first row of its next tile.
 template <int DT, int G, int TW> struct Walk {
     using L = Place<DT, G, TW>;
     using T = typename L::T;
-    static constexpr int CPR = L::RB / 16, RPI = 32 / CPR;   // 16-byte chunks of a row; rows of one instruction
-    static_assert(RPI % TW == 0 || TW % RPI == 0, "an instruction's rows are whole slots or part of one");
+    static constexpr int ES = sizeof(T);
     char *at;
-    int64_t step, lane_off, rows_off;   // bytes: from tile to tile, to the lane's chunk, from one instruction's rows to the next's
-    int64_t ls;
-    __device__ __forceinline__ Walk(const void *base, int64_t bs, int64_t ls_, const L &p, int row, int64_t rows_per_step) : ls(ls_) {
-        at = (char *)base + (p.b * bs + row * ls + p.c0) * (int64_t)sizeof(T);
-        step = rows_per_step * ls * (int64_t)sizeof(T);
-        lane_off = (p.lane / CPR) * ls * (int64_t)sizeof(T) + p.lane % CPR * 16;
-        rows_off = RPI * ls * (int64_t)sizeof(T);
+    int64_t step, row;   // bytes: from tile to tile, from row to row
+    __device__ __forceinline__ Walk(const void *base, int64_t bs, int64_t ls, const L &p, int first, int64_t rows_per_step)
+        : at((char *)base + (p.b * bs + first * ls + p.c0) * (int64_t)ES), step(rows_per_step * ls * ES), row(ls * ES) {}
+    // Pieces of B bytes: a warp moves RPI rows at a time, in N instructions where a row has more than 32 pieces.
+    template <int B> struct Pieces {
+        static constexpr int CPR = L::RB / B, N = CPR > 32 ? CPR / 32 : 1, RPI = CPR > 32 ? 1 : 32 / CPR;
+        static_assert(RPI % TW == 0 || TW % RPI == 0, "an instruction's rows are whole slots or part of one");
+        static __device__ __forceinline__ int of(int lane) { return CPR > 32 ? lane : lane % CPR; }
+        static __device__ __forceinline__ int row(int lane) { return CPR > 32 ? 0 : lane / CPR; }
+        static __device__ __forceinline__ int place(int j) { return RPI >= TW ? j * (RPI / TW) * L::SB : j * RPI / TW * L::SB + j * RPI % TW * L::RB; }
+        static __device__ __forceinline__ int lane_place(int lane) { return row(lane) / TW * L::SB + row(lane) % TW * L::RB + of(lane) * B; }
+    };
+    template <int B> __device__ __forceinline__ void fetch_pieces(unsigned char *dst, int n, const L &p, int dim) const {
+        using Q = Pieces<B>;
+        const char *s = at + Q::row(p.lane) * row + Q::of(p.lane) * B;
+        unsigned char *d = dst + Q::lane_place(p.lane);
+        const int64_t rows = Q::RPI * row;
+        if (n == L::ROWS && p.full) {
+#pragma unroll
+            for (int j = 0; j < L::ROWS / Q::RPI; ++j) {
+#pragma unroll
+                for (int h = 0; h < Q::N; ++h) copy_async<B>(d + Q::place(j) + h * 32 * B, s + h * 32 * B);
+                s += rows;
+            }
+        } else {   // what is not there comes as zeros
+            const int left = n - Q::row(p.lane), c = p.c0 + Q::of(p.lane) * B / ES;
+#pragma unroll
+            for (int j = 0; j < L::ROWS / Q::RPI; ++j) {
+#pragma unroll
+                for (int h = 0; h < Q::N; ++h) {
+                    const bool ok = j * Q::RPI < left && c + h * 32 * B / ES < dim;
+                    copy_async<B>(d + Q::place(j) + h * 32 * B, ok ? s + h * 32 * B : at, ok);
+                }
+                s += rows;
+            }
+        }
     }
-    static __device__ __forceinline__ int place(int j) { return RPI >= TW ? j * (RPI / TW) * L::SB : j * RPI / TW * L::SB + j * RPI % TW * L::RB; }
-    static __device__ __forceinline__ int lane_place(const L &p) { const int r0 = p.lane / CPR; return r0 / TW * L::SB + r0 % TW * L::RB + p.lane % CPR * 16; }
-    // The n rows that are there to shared memory; what is not comes as zeros.
+    template <int B> __device__ __forceinline__ void flush_pieces(const unsigned char *tile, int n, const L &p, int dim) const {
+        using Q = Pieces<B>;
+        using W = typename WordOf<B>::W;
+        char *d = at + Q::row(p.lane) * row + Q::of(p.lane) * B;
+        const unsigned char *s = tile + Q::lane_place(p.lane);
+        const int64_t rows = Q::RPI * row;
+        const int left = n - Q::row(p.lane), c = p.c0 + Q::of(p.lane) * B / ES;
+#pragma unroll
+        for (int j = 0; j < L::ROWS / Q::RPI; ++j) {
+#pragma unroll
+            for (int h = 0; h < Q::N; ++h)
+                if (j * Q::RPI < left && c + h * 32 * B / ES < dim) *(W *)(d + h * 32 * B) = *(const W *)(s + Q::place(j) + h * 32 * B);
+            d += rows;
+        }
+    }
+    // The n rows that are there to shared memory.
     __device__ __forceinline__ void fetch(unsigned char *dst, int n, const L &p, int dim, int how) const {
-        if (how == GS_CHUNKS) {
-            const char *s = at + lane_off;
-            unsigned char *d = dst + lane_place(p);
-            if (n == L::ROWS && p.full) {
-#pragma unroll
-                for (int j = 0; j < L::ROWS / RPI; ++j) {
-                    copy_async<16>(d + place(j), s);
-                    s += rows_off;
-                }
-            } else {
-                const int left = p.c0 + p.lane % CPR * (16 / (int)sizeof(T)) < dim ? n - p.lane / CPR : 0;
-#pragma unroll
-                for (int j = 0; j < L::ROWS / RPI; ++j) {
-                    copy_async<16>(d + place(j), s, j * RPI < left);
-                    if ((j + 1) * RPI < left) s += rows_off;   // stays inside the tensor where it was
-                }
-            }
-        } else if (how == GS_WORDS) {
-            constexpr int WPR = L::RB / 4;
-#pragma unroll 4
-            for (int j = p.lane; j < L::ROWS * WPR; j += 32) {
-                const int r = j / WPR, w = j % WPR;
-                const bool ok = p.c0 + w * (4 / (int)sizeof(T)) < dim && r < n;
-                copy_async<4>(dst + r / TW * L::SB + r % TW * L::RB + w * 4, ok ? at + r * ls * (int64_t)sizeof(T) + w * 4 : at, ok);
-            }
-        } else if constexpr (sizeof(T) == 2) {
+        if (how == GS_CHUNKS) fetch_pieces<16>(dst, n, p, dim);
+        else if (how == GS_WORDS) fetch_pieces<4>(dst, n, p, dim);
+        else if constexpr (ES == 2) {
             T *d = (T *)(dst + p.sub * L::SB) + p.li * 2;
-            const T *s = (const T *)at + p.sub * TW * ls + (p.ch - p.c0);
+            const char *s = at + p.sub * TW * row + (p.ch - p.c0) * ES;
 #pragma unroll 4
             for (int i = 0; i < TW; ++i) {
                 const bool ok = p.sub * TW + i < n;
-                d[i * L::CB] = ok && p.one ? s[i * ls] : Elem<DT>::down(0.f);
-                d[i * L::CB + 1] = ok && p.two ? s[i * ls + 1] : Elem<DT>::down(0.f);
+                d[i * L::CB] = ok && p.one ? ((const T *)(s + i * row))[0] : Elem<DT>::down(0.f);
+                d[i * L::CB + 1] = ok && p.two ? ((const T *)(s + i * row))[1] : Elem<DT>::down(0.f);
             }
         }
     }
     // The first n rows of a staged tile to the tensor.
     __device__ __forceinline__ void flush(const unsigned char *tile, int n, const L &p, int dim, int how) const {
-        if (how == GS_CHUNKS) {
-            char *d = at + lane_off;
-            const unsigned char *s = tile + lane_place(p);
-            const int left = p.c0 + p.lane % CPR * (16 / (int)sizeof(T)) < dim ? n - p.lane / CPR : 0;
-#pragma unroll
-            for (int j = 0; j < L::ROWS / RPI; ++j) {
-                if (j * RPI < left) *(uint4 *)d = *(const uint4 *)(s + place(j));
-                d += rows_off;
-            }
-        } else {
+        if (how == GS_CHUNKS) flush_pieces<16>(tile, n, p, dim);
+        else if (how == GS_WORDS) flush_pieces<4>(tile, n, p, dim);
+        else if constexpr (ES == 2) {
 #pragma unroll 1
             for (int j = p.lane; j < L::ROWS * L::CB; j += 32) {
                 const int r = j / L::CB, c = j % L::CB;
-                if (r < n && p.c0 + c < dim) ((T *)at)[r * ls + c] = ((const T *)(tile + r / TW * L::SB + r % TW * L::RB))[c];
+                if (r < n && p.c0 + c < dim) ((T *)(at + r * row))[c] = ((const T *)(tile + r / TW * L::SB + r % TW * L::RB))[c];
             }
         }
     }
