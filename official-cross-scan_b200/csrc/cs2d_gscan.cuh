@@ -9,6 +9,7 @@
 
 #include <cooperative_groups.h>
 
+#include <algorithm>
 #include <cstring>
 
 #include "cs2d_seq.cuh"
@@ -19,7 +20,7 @@ namespace gs {
 
 namespace cg = cooperative_groups;
 
-constexpr int MAXC = 8;        // CTAs of a cluster, at most
+constexpr int MAXC = 16;       // CTAs of a cluster, at most
 constexpr int NW = 8;          // warps of a CTA
 
 __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) { return __ffma2_rn(a, b, c); }
@@ -336,8 +337,7 @@ template <bool GROWS, bool PACKED, bool UP, int G, class Place>
 __device__ __forceinline__ float2 pass_cluster(const MapStore<G> *maps, Exchange<G> *x, unsigned step, int rank, int C, const Place &at, float2 &state,
                                                int *status) {
     const int place = step & 1;
-    if (at.warp < C) {   // warp r sends to CTA r
-        const int r = at.warp;
+    for (int r = at.warp; r < C; r += NW) {   // warp r sends to CTA r (and r + 8)
         Map<GROWS, PACKED> m;
 #pragma unroll
         for (int k = 0; k < NW; ++k) {
@@ -370,44 +370,62 @@ __device__ __forceinline__ float2 pass_cluster(const MapStore<G> *maps, Exchange
         }
     }
     if (threadIdx.x == 0) expect<PACKED>(x, place, C);
-    float2 own = pass<GROWS, PACKED, UP, MAXC>(x->slot[place], C, rank, at.li, state);
+    float2 own = state;
+#pragma unroll 4
+    for (int k = 0; k < C; ++k) {
+        const int r = UP ? k : C - 1 - k;
+        if (r == rank) own = state;
+        state = x->slot[place][r].template get<GROWS, PACKED>(at.li).apply(state);
+    }
     return pass<GROWS, PACKED, UP, NW>(maps, NW, at.wi, at.li, own);
 }
 
 // ---- launches ----------------------------------------------------------------------------------------------------
-static_assert(MAXC <= NW, "a warp per receiver");
-struct Split { int wt, C; int64_t grid; };
+struct Split { int wt, C; int64_t grid; };   // warps along the rows; CTAs of a cluster
 
-template <class K> cudaError_t start(K *kernel, const GScan &P, const Split &s, size_t smem, cudaStream_t st) {
-    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-    if (e != cudaSuccess) return e;
-    cudaLaunchConfig_t cfg = {};
-    cudaLaunchAttribute attr[1];
-    cfg.gridDim = dim3((unsigned)s.grid);
+inline void configure(cudaLaunchConfig_t &cfg, cudaLaunchAttribute *attr, int64_t grid, int C, size_t smem, cudaStream_t st) {
+    cfg = {};
+    cfg.gridDim = dim3((unsigned)grid);
     cfg.blockDim = dim3(32 * NW);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = st;
-    if (s.C > 1) {
-        attr[0].id = cudaLaunchAttributeClusterDimension;
-        attr[0].val.clusterDim.x = s.C;
-        attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-        cfg.attrs = attr;
-        cfg.numAttrs = 1;
-    }
-    return cudaLaunchKernelEx(&cfg, kernel, P, s.wt, s.C);
+    if (C == 1) return;
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = C;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
 }
-
-// How the rows are split over warps and CTAs; rows: of a warp's tile.  Two CTAs fit an SM (128 registers per thread); with fewer than 192 of them
-// the rows are split over a cluster.
-inline Split split(GScan &P, int G, int rows) {
+// Launches KERNEL with its rows split as they should be; rows: of a warp's tile.
+template <auto KERNEL> cudaError_t start(GScan &P, int G, int rows, size_t smem, cudaStream_t st) {
+    static int at_once[64][MAXC + 1] = {};   // per device and cluster size: clusters that fit the GPU at a time
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess || dev < 0 || dev >= 64) return e != cudaSuccess ? e : cudaErrorInvalidDevice;
+    cudaLaunchConfig_t cfg;
+    cudaLaunchAttribute attr[1];
+    if (!at_once[dev][1]) {
+        if ((e = cudaFuncSetAttribute(KERNEL, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem)) != cudaSuccess) return e;
+        if ((e = cudaFuncSetAttribute(KERNEL, cudaFuncAttributeNonPortableClusterSizeAllowed, 1)) != cudaSuccess) return e;
+        for (int C = MAXC; C >= 1; --C) {
+            configure(cfg, attr, C, C, smem, st);
+            if (C == 1) at_once[dev][C] = 1;
+            else if (cudaOccupancyMaxActiveClusters(&at_once[dev][C], KERNEL, &cfg) != cudaSuccess) at_once[dev][C] = 0;
+        }
+        cudaGetLastError();   // (a size that the device does not have)
+    }
     Split s{1, 1, 0};
     P.nblk = (P.dim + 2 * G - 1) / (2 * G);
     P.units = (int64_t)P.batch * P.nblk;
-    while (s.wt < NW && (int64_t)s.wt * rows < P.length) s.wt <<= 1;
+    while (s.wt < NW && (int64_t)s.wt * rows < P.length) s.wt <<= 1;   // the others take further units
     const int64_t tile = (int64_t)s.wt * rows, tiles = (P.length + tile - 1) / tile, per = NW / s.wt, ctas = (P.units + per - 1) / per;
-    while (s.C < MAXC && s.C < tiles && ctas * s.C < 192) s.C <<= 1;
+    // The largest cluster of which all fit the GPU at once: a second round would take as long as the first (24 units: 26 clusters of 10
+    // fit, B1 L67200 D384 70 + 115 us; 21 of 12, 90 + 148 us; 33 of 8, 78 + 129 us).
+    for (int C = (int)(tiles < MAXC ? tiles : MAXC); C > 1 && s.C == 1; --C)
+        if (at_once[dev][C] >= ctas) s.C = C;
     s.grid = ctas * s.C;
-    return s;
+    configure(cfg, attr, s.grid, s.C, smem, st);
+    return cudaLaunchKernelEx(&cfg, KERNEL, (const GScan)P, (const int)s.wt, (const int)s.C);
 }
 // Units of 16 channels instead of 64 where the wide ones would not fill the GPU: rows of 32 bytes instead of 128 are read a little slower (bf16,
 // B16 L16384 D512: 252 + 411 us instead of 184 + 376), but there are four times as many units (B1 L67200 D384: 84 + 150 us instead of 214 + 435;

@@ -188,9 +188,8 @@ __global__ void __launch_bounds__(32 * NW, 2) gscan_bwd(const GScan P, const int
 }
 
 template <int DT, int G, int FORM, bool WEIGHTED> cudaError_t bwd3(GScan P, cudaStream_t st) {
-    const Split s = split(P, G, Place<DT, G, BTW<DT>>::ROWS);
-    const size_t smem = bwd_smem<DT, G>();
-    return P.map ? start(gscan_bwd<DT, G, FORM, WEIGHTED, true>, P, s, smem, st) : start(gscan_bwd<DT, G, FORM, WEIGHTED, false>, P, s, smem, st);
+    constexpr int rows = Place<DT, G, BTW<DT>>::ROWS;
+    return P.map ? start<gscan_bwd<DT, G, FORM, WEIGHTED, true>>(P, G, rows, bwd_smem<DT, G>(), st) : start<gscan_bwd<DT, G, FORM, WEIGHTED, false>>(P, G, rows, bwd_smem<DT, G>(), st);
 }
 template <int DT, int G> cudaError_t bwd2(const GScan &P, cudaStream_t st) {
     switch (P.form * 2 + P.weighted) {
