@@ -9,7 +9,6 @@
 
 #include <cooperative_groups.h>
 
-#include <algorithm>
 #include <cstring>
 
 #include "cs2d_seq.cuh"

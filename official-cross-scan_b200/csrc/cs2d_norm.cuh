@@ -533,26 +533,30 @@ __global__ void __launch_bounds__(NT, (BWD_CTAS<DT, V, NV, GATED>)) norm_bwd(con
 }
 
 // ---- launches ----------------------------------------------------------------------------------------------------
-template <class K> cudaError_t start(K *kernel, const Norm &P, const Layout &l, size_t smem, cudaStream_t st) {
+template <auto KERNEL> cudaError_t start(const Norm &P, const Layout &l, size_t smem, cudaStream_t st) {
+    static bool done[64] = {};   // per device
     const size_t acc = (size_t)8 * P.dim;   // the backward's sums, in the place of all else
     if (P.dy && smem < acc) smem = acc;
-    if (smem > 40 * 1024) {   // the default limit counts static shared memory too
-        const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-        if (e != cudaSuccess) return e;
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess || dev < 0 || dev >= 64) return e != cudaSuccess ? e : cudaErrorInvalidDevice;
+    if (!done[dev]) {
+        if ((e = cudaFuncSetAttribute(KERNEL, cudaFuncAttributeMaxDynamicSharedMemorySize, 226 * 1024)) != cudaSuccess) return e;
+        done[dev] = true;
     }
-    kernel<<<l.grid, NT, smem, st>>>(P, l);
+    KERNEL<<<l.grid, NT, smem, st>>>(P, l);
     return cudaGetLastError();
 }
 template <bool BWD, int DT, int V, int NV> cudaError_t go(const Norm &P, const Layout &l, size_t smem, cudaStream_t st) {
     const bool image = l.image;
     if constexpr (BWD) {
-        if (P.gate) return image ? start(norm_bwd<DT, V, NV, true, true>, P, l, smem + 2 * STAGE_BYTES<V, NV, true, true>, st)
-                                 : start(norm_bwd<DT, V, NV, true, false>, P, l, smem + 2 * STAGE_BYTES<V, NV, true, false>, st);
-        return image ? start(norm_bwd<DT, V, NV, false, true>, P, l, smem + 2 * STAGE_BYTES<V, NV, false, true>, st)
-                     : start(norm_bwd<DT, V, NV, false, false>, P, l, smem + 2 * STAGE_BYTES<V, NV, false, false>, st);
+        if (P.gate) return image ? start<norm_bwd<DT, V, NV, true, true>>(P, l, smem + 2 * STAGE_BYTES<V, NV, true, true>, st)
+                                 : start<norm_bwd<DT, V, NV, true, false>>(P, l, smem + 2 * STAGE_BYTES<V, NV, true, false>, st);
+        return image ? start<norm_bwd<DT, V, NV, false, true>>(P, l, smem + 2 * STAGE_BYTES<V, NV, false, true>, st)
+                     : start<norm_bwd<DT, V, NV, false, false>>(P, l, smem + 2 * STAGE_BYTES<V, NV, false, false>, st);
     } else {
-        if (P.gate) return image ? start(norm_fwd<DT, V, NV, true, true>, P, l, smem, st) : start(norm_fwd<DT, V, NV, true, false>, P, l, smem, st);
-        return image ? start(norm_fwd<DT, V, NV, false, true>, P, l, smem, st) : start(norm_fwd<DT, V, NV, false, false>, P, l, smem, st);
+        if (P.gate) return image ? start<norm_fwd<DT, V, NV, true, true>>(P, l, smem, st) : start<norm_fwd<DT, V, NV, true, false>>(P, l, smem, st);
+        return image ? start<norm_fwd<DT, V, NV, false, true>>(P, l, smem, st) : start<norm_fwd<DT, V, NV, false, false>>(P, l, smem, st);
     }
 }
 template <bool BWD, int DT> cudaError_t launch(const Norm &P, const Layout &l, int v, int nv, size_t smem, cudaStream_t st) {
@@ -560,7 +564,7 @@ template <bool BWD, int DT> cudaError_t launch(const Norm &P, const Layout &l, i
     if (v == V) switch (nv) {
             case 1: return go<BWD, DT, V, 1>(P, l, smem, st);
             case 2: return go<BWD, DT, V, 2>(P, l, smem, st);
-            case 3: if constexpr (BWD) return P.gate || l.image ? cudaErrorInvalidValue : start(norm_bwd<DT, V, 3, false, false>, P, l, smem + 2 * STAGE_BYTES<V, 3, false, false>, st);
+            case 3: if constexpr (BWD) return P.gate || l.image ? cudaErrorInvalidValue : start<norm_bwd<DT, V, 3, false, false>>(P, l, smem + 2 * STAGE_BYTES<V, 3, false, false>, st);
                     else return go<BWD, DT, V, 3>(P, l, smem, st);
             case 6: if constexpr (DT == CS2D_F32 && !BWD) return go<BWD, DT, V, 6>(P, l, smem, st);
         }

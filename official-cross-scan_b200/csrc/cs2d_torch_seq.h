@@ -260,11 +260,14 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
         const auto o = [&](int i) { return given(s[i]) ? OptT(s[i]) : OptT(); };
         const NormArgs a = norm_args(s[0], o(1), o(2), o(3), ctx->saved_data["eps"].toDouble());
         const c10::cuda::CUDAGuard guard(a.x.device());
-        Tensor dw, db, dz;
-        if (given(a.weight)) dw = at::empty(a.weight.sizes(), a.weight.options());
-        if (given(a.bias)) db = at::empty(a.bias.sizes(), a.bias.options());
+        Tensor dw, db, dz, scratch;
+        const auto parameters = [&]() {
+            if (given(a.weight)) dw = at::empty(a.weight.sizes(), a.weight.options());
+            if (given(a.bias)) db = at::empty(a.bias.sizes(), a.bias.options());
+        };
         if (given(a.gate)) dz = at::empty(a.gate.sizes(), a.gate.options());
         if (a.x.numel() == 0) {
+            parameters();
             if (given(dw)) dw.zero_();
             if (given(db)) db.zero_();
             return {at::empty(a.x.sizes(), a.x.options()), dw, db, dz, Tensor()};
@@ -288,7 +291,15 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
         }
         const size_t nbytes = cs2d_norm_bwd_scratch_bytes(&p);
         CS2D_CHECK(nbytes != 0, "cs2d layer norm: ", cs2d_last_error());
-        const Tensor scratch = f32(a.x, (int64_t)(nbytes / 4));
+        const int64_t ns = (int64_t)(nbytes / 4), d4 = (p.dim + 3) / 4 * 4;
+        if (p.param_dtype == CS2D_F32 && ns + 2 * d4 <= (1 << 16)) {   // small problems: one allocation (what a caller keeps keeps no more than 256 KB alive)
+            scratch = f32(a.x, ns + 2 * d4);
+            if (given(a.weight)) dw = part_of(scratch, ns, {p.dim});
+            if (given(a.bias)) db = part_of(scratch, ns + d4, {p.dim});
+        } else {
+            parameters();
+            scratch = f32(a.x, ns);
+        }
         raise_on(cs2d_norm_bwd(&p, dy.const_data_ptr(), r.os, r.is, s[4].const_data_ptr<float>(), scratch.data_ptr(), dx.data_ptr(), os, is, cs,
                                given(dz) ? dz.data_ptr() : nullptr, given(dw) ? dw.data_ptr() : nullptr, given(db) ? db.data_ptr() : nullptr,
                                stream_of(a.x)), "layer norm backward");

@@ -211,6 +211,32 @@ def test_empty_and_refusals():
         torch.autograd.grad(cs2d.layer_norm(x).sum(), x, create_graph=True)
 
 
+def test_first_calls_of_a_process_inside_a_capture():
+    """Nothing has been launched before: the recorded step prepares its kernels itself."""
+    import subprocess
+    import sys
+    from conftest import ROOT
+    code = """
+import sys, torch
+sys.path.insert(0, "official-cross-scan_b200")
+import cs2d
+u, g, z = (torch.randn(1, 700, 64, device="cuda") for _ in range(3))
+w = torch.ones(64, device="cuda")
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    a = [t.requires_grad_(True) for t in (u, g, z, w)]
+    y = cs2d.layer_norm(cs2d.gated_scan_1d(a[0], a[1])[0], a[3], None, a[2])
+    grads = torch.autograd.grad(y, a, torch.ones_like(y))
+graph.replay()
+torch.cuda.synchronize()
+kept = [t.clone() for t in (y, *grads)]
+y = cs2d.layer_norm(cs2d.gated_scan_1d(a[0], a[1])[0], a[3], None, a[2])
+print(all(torch.equal(p, q) for p, q in zip(kept, (y, *torch.autograd.grad(y, a, torch.ones_like(y))))))
+"""
+    r = subprocess.run([sys.executable, "-c", code], cwd=ROOT, capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and r.stdout.split() == ["True"], r.stdout + r.stderr
+
+
 def test_same_bits_every_time_on_other_streams_and_from_a_graph():
     for image in (False, True):
         d = inputs((4, 30, 31), 192, BF16, image=image)
