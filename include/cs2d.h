@@ -264,7 +264,7 @@ int cs2d_bwd_noalloc(const cs2d_problem *p, const void *dout, int64_t dout_bs, i
  * with a from the gate by `form` (CS2D_GATE_SIGMOID: 1 / (1 + exp(-gate)), CS2D_GATE_LOG: exp(gate),
  * CS2D_GATE_DIRECT: gate) and b = u, or (1 - a) * u where `weighted` is set.  The state is fp32 throughout; y is
  * rounded to the input type once per element.  Factors above one are allowed as long as the product of
- * 256 consecutive ones stays inside the range of fp32.
+ * 512 consecutive ones stays inside the range of fp32.
  *
  * u, gate (batch, length, dim) of io_dtype, channel stride 1, other strides in elements.  h0 (states, dim) fp32, rows
  * h0_bs apart, or NULL (zeros).  Without `offsets` there are `batch` states.  With them batch is 1 and `offsets`
@@ -315,7 +315,7 @@ int cs2d_gscan_step(const cs2d_gscan *p, void *y, int64_t y_bs, float *h, int64_
  *     y = ((x - mean) / sqrt(var + eps) * weight + bias) * silu(gate)
  * Row (o, i), 0 <= o < outer, 0 <= i < inner, channel d is x[o * x_os + i * x_is + d * x_cs]; x_cs (rows of tokens) or x_is
  * (channel-major images) must be 1.  gate: channel stride 1, or NULL.  weight, bias (dim) of param_dtype (fp32 or the
- * input type), dense, or NULL (ones, zeros).  y (outer, inner, dim) of io_dtype, dense.  stats (outer * inner, 2) fp32 receives mean
+ * input type), dense, or NULL (ones, zeros).  y (outer, inner, dim) of io_dtype, dense.  stats (outer * inner, 2) fp32, 8-byte aligned, receives mean
  * and 1 / sqrt(var + eps) for the backward, or NULL.  Sums and statistics are fp32, the variance that of the centred values.
  */
 typedef struct {

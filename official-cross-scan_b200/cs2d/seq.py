@@ -13,7 +13,7 @@ per channel, with the factor ``a`` from the gate and the input term ``b`` from `
 ===========  ==========================  =====================
 
 and ``b = u`` otherwise.  The state is float32 throughout, whatever the type of ``u`` and ``gate``; ``y`` is rounded once
-per element.  Factors above one are allowed as long as the product of 256 consecutive ones stays inside float32.
+per element.  Factors above one are allowed as long as the product of 512 consecutive ones stays inside float32.
 Results and gradients come out with the same bits on every run.  As everywhere in this package there is no CPU or
 PyTorch fallback.
 """

@@ -314,7 +314,7 @@ template <int G> struct Exchange {
     MapStore<G> slot[2][MAXC];
     uint64_t full[2], pad[2];
 };
-constexpr int WAIT_POLLS = 1 << 22;
+constexpr int WAIT_POLLS = 1 << 20;
 __device__ __forceinline__ unsigned shared_address(const void *p) { return (unsigned)__cvta_generic_to_shared(p); }
 template <bool PACKED, int G> __device__ __forceinline__ void expect(Exchange<G> *x, int place, int C) {   // one thread
     asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(shared_address(&x->full[place])), "r"(C * (G * 16 + (PACKED ? 4 : 0))) : "memory");

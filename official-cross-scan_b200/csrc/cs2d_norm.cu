@@ -162,11 +162,11 @@ Plan plan(const Norm &P, int dt, bool bwd) {
     if (image) {
         const int64_t row = (int64_t)P.dim * es;
         r.l.pitch = (int)(es == 2 ? (row + 63) / 128 * 128 + 64 : (row + 127) / 128 * 128 + 16);
-        r.l.P = es == 2 ? 64 : 32;   // 128 bytes of a channel
-        while (r.l.P > 16 && (P.inner + r.l.P - 1) / r.l.P * (P.rows / P.inner) < 2 * kSMs) r.l.P >>= 1;
+        r.l.whole = P.inner * es % 16 == 0 && on16(P.x, P.x_os, P.x_cs, es) && (!bwd || on16(P.dx, P.dx_os, P.dx_cs, es));
+        r.l.P = es == 2 ? 64 : 32;   // 128 bytes of a channel; fewer where there would be few tiles, or where two CTAs would not fit an SM
+        while (r.l.P > (r.l.whole && es == 2 ? 32 : 16) && (P.inner + r.l.P - 1) / r.l.P * (P.rows / P.inner) < 2 * kSMs) r.l.P >>= 1;
         while (r.l.P > 8 && r.l.P * (int64_t)r.l.pitch > (bwd ? 56 : 72) * 1024) r.l.P >>= 1;
         if (r.l.P * (int64_t)r.l.pitch > (bwd ? 120 : 220) * 1024) r.wide = true;
-        r.l.whole = P.inner * es % 16 == 0 && on16(P.x, P.x_os, P.x_cs, es) && (!bwd || on16(P.dx, P.dx_os, P.dx_cs, es));
         r.smem = (size_t)r.l.P * r.l.pitch;
     } else {   // some rows per group and tile, as long as there are tiles for all CTAs
         int k = 8;

@@ -89,6 +89,7 @@ size_t cs2d_gscan_saved_bytes(const cs2d_gscan *p, int keep) {
 int cs2d_gscan_fwd(const cs2d_gscan *p, void *y, int64_t y_bs, int64_t y_ls, float *h_last, void *saved, int keep, void *stream) {
     if (const int rc = validate(p, false)) return rc;
     if (!y || !saved || (!h_last && !(p->offsets && p->n_seq == 0))) return fail(CS2D_ERR_INVALID, "y, h_last and saved must be given");
+    if (reinterpret_cast<uintptr_t>(saved) % 16) return fail(CS2D_ERR_INVALID, "saved must be 16-byte aligned");
     GScan d;
     if (const int rc = fill(d, p, saved)) return rc;
     const int es = p->io_dtype == CS2D_F32 ? 4 : 2;
@@ -106,6 +107,7 @@ int cs2d_gscan_bwd(const cs2d_gscan *p, const void *dy, int64_t dy_bs, int64_t d
                    const void *saved, void *du, void *dgate, float *dh0, void *stream) {
     if (const int rc = validate(p, false)) return rc;
     if (!dy || !saved || !du || !dgate) return fail(CS2D_ERR_INVALID, "dy, saved, du and dgate must be given");
+    if (reinterpret_cast<uintptr_t>(saved) % 16) return fail(CS2D_ERR_INVALID, "saved must be 16-byte aligned");
     GScan d;
     if (const int rc = fill(d, p, const_cast<void *>(saved))) return rc;
     const int es = p->io_dtype == CS2D_F32 ? 4 : 2;
@@ -129,6 +131,7 @@ int cs2d_gscan_step(const cs2d_gscan *p, void *y, int64_t y_bs, float *h, int64_
 int cs2d_norm_fwd(const cs2d_norm *p, void *y, float *stats, void *stream) {
     if (const int rc = validate(p)) return rc;
     if (!y) return fail(CS2D_ERR_INVALID, "y must be given");
+    if (reinterpret_cast<uintptr_t>(stats) % 8) return fail(CS2D_ERR_INVALID, "stats must be 8-byte aligned");
     Norm d = fill(p);
     d.y = y; d.stats = stats;
     return launched(launch_norm_fwd(d, p->io_dtype, static_cast<cudaStream_t>(stream)), 1);
@@ -143,6 +146,7 @@ int cs2d_norm_bwd(const cs2d_norm *p, const void *dy, int64_t dy_os, int64_t dy_
                   int64_t dx_os, int64_t dx_is, int64_t dx_cs, void *dgate, void *dweight, void *dbias, void *stream) {
     if (const int rc = validate(p)) return rc;
     if (!dy || !stats || !dx || !scratch || (p->gate && !dgate)) return fail(CS2D_ERR_INVALID, "dy, stats, scratch, dx and the gate's gradient must be given");
+    if (reinterpret_cast<uintptr_t>(stats) % 8 || reinterpret_cast<uintptr_t>(scratch) % 16) return fail(CS2D_ERR_INVALID, "stats must be 8-byte, scratch 16-byte aligned");
     if (dx_cs != 1 && dx_is != 1) return fail(CS2D_ERR_INVALID, "dx must have stride 1 along its channels or its rows");
     Norm d = fill(p);
     d.dy = dy; d.dy_os = dy_os; d.dy_is = dy_is; d.stats = const_cast<float *>(stats); d.part = (float *)scratch;
