@@ -5,6 +5,13 @@
 // that reaches it.  A warp copies its own rows to shared memory some tiles ahead (16 bytes per lane and copy), keeps the factors in
 // registers between the two walks, and writes each result once: every input is read once and every output written once.  A lane holds two
 // channels, which one packed instruction serves.  Nothing depends on the order in which CTAs run.
+//
+// Units are 64 channels wide (rows of 128 bytes of a 16-bit type) or, where those would not fill the GPU, 16 (a warp then holds four slots of rows).
+// Eight warps to a CTA, two CTAs to an SM: one computes while the other waits at its barrier (one CTA of 16 warps: 10 % slower).
+// What bounds it is the issue of instructions, not memory: 24 per element and warp lane in the forward, 49 in the backward (sigmoid gate, ncu),
+// 50 % of the issue slots used, the rest waits for MUFU results, shared memory and the barrier.  Measured (bf16, sigmoid, kernels
+// alone): B16 L16384 D512 forward 184 us, 67 % of the HBM copy rate, backward 360 us, 57 %; B8 L4096 D768 53 + 96 us (192 CTAs on 296 places);
+// B1 L67200 D384 70 + 115 us.
 #pragma once
 
 #include <cooperative_groups.h>
