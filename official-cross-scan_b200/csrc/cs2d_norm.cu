@@ -128,8 +128,8 @@ __global__ void __launch_bounds__(1024) norm_join(const Norm P) {
 
 // Lanes of a row and vectors of a lane: the fewest places for the row's vectors, of equal ones the fewest lanes (fewer shuffles).
 bool lanes_of(int dim, int v, int dt, bool bwd, bool heavy, int *T, int *nv) {
-    static const int two[] = {1, 2, 0}, three[] = {1, 2, 3, 0}, f32[] = {1, 2, 3, 6, 0}, single[] = {4, 12, 24, 0};
-    const int *set = v == 1 ? single : bwd ? (heavy ? two : three) : dt == CS2D_F32 ? f32 : three;
+    static const int two[] = {1, 2, 0}, three[] = {1, 2, 3, 0}, f32[] = {1, 2, 3, 6, 0}, pairs[] = {2, 4, 6, 0}, single[] = {4, 6, 8, 12, 0};
+    const int *set = v == 1 ? single : v == 2 ? pairs : bwd ? (heavy ? two : three) : dt == CS2D_F32 ? f32 : three;
     const int nvec = dim / v;
     int best = 0;
     for (int t = 1; t <= nm::NT; t <<= 1)
@@ -140,7 +140,8 @@ bool lanes_of(int dim, int v, int dt, bool bwd, bool heavy, int *T, int *nv) {
         }
     return best != 0;
 }
-bool on16(const void *p, int64_t a, int64_t b, int es) { return reinterpret_cast<uintptr_t>(p) % 16 == 0 && a * es % 16 == 0 && b * es % 16 == 0; }
+bool on(int bytes, const void *p, int64_t a, int64_t b, int es) { return reinterpret_cast<uintptr_t>(p) % bytes == 0 && a * es % bytes == 0 && b * es % bytes == 0; }
+bool on16(const void *p, int64_t a, int64_t b, int es) { return on(16, p, a, b, es); }
 
 struct Plan { nm::Layout l; int v, nv; size_t smem; bool wide; };
 constexpr int kSMs = 148;
@@ -149,15 +150,21 @@ Plan plan(const Norm &P, int dt, bool bwd) {
     Plan r{};
     const int es = dt == CS2D_F32 ? 4 : 2, V = 16 / es;
     const bool image = P.x_cs != 1;
-    bool vec = P.dim % V == 0 && on16(P.y, 0, 0, es) && (!P.gate || on16(P.gate, P.g_os, P.g_is, es)) && on16(P.weight, 0, 0, 1) && on16(P.bias, 0, 0, 1);
-    if (!image) vec = vec && on16(P.x, P.x_os, P.x_is, es);
-    if (bwd) vec = vec && on16(P.dy, P.dy_os, P.dy_is, es) && on16(P.dgate, 0, 0, es) && (image || on16(P.dx, P.dx_os, P.dx_is, es));
-    r.v = vec ? V : 1;
+    // vectors of 16 bytes, pairs of 16-bit elements, single elements
+    const auto fits = [&](int v) {
+        const int n = v * es;
+        bool ok = P.dim % v == 0 && on(n, P.y, 0, 0, es) && (!P.gate || on(n, P.gate, P.g_os, P.g_is, es)) && (v == 2 || (on16(P.weight, 0, 0, 1) && on16(P.bias, 0, 0, 1)));
+        if (v == 2 && P.wtype != CS2D_F32) ok = ok && on(4, P.weight, 0, 0, 1) && on(4, P.bias, 0, 0, 1);
+        if (!image) ok = ok && on(n, P.x, P.x_os, P.x_is, es);
+        if (bwd) ok = ok && on(n, P.dy, P.dy_os, P.dy_is, es) && on(n, P.dgate, 0, 0, es) && (image || on(n, P.dx, P.dx_os, P.dx_is, es));
+        return ok;
+    };
+    r.v = fits(V) ? V : es == 2 && fits(2) ? 2 : 1;
     r.wide = !lanes_of(P.dim, r.v, dt, bwd, P.gate || image, &r.l.T, &r.nv);
     // images whose gradient is not one, and the other way round, take the wide kernels too
     if (bwd && image != (P.dx_cs != 1)) r.wide = true;
     if (r.wide) return r;
-    const int e = r.v * r.nv, per = bwd ? (e <= 8 ? 4 : e <= 12 && r.v > 1 ? 3 : 2) : 6, groups = nm::NT / r.l.T;
+    const int e = r.v * r.nv, per = bwd ? (r.v == 1 ? 2 : e <= 8 ? 4 : e <= 12 ? 3 : 2) : 6, groups = nm::NT / r.l.T;
     r.l.image = image;
     if (image) {
         const int64_t row = (int64_t)P.dim * es;

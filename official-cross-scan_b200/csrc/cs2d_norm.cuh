@@ -84,10 +84,10 @@ template <int DT, int V, int NV> struct Row {
         } else {
 #pragma unroll
             for (int j = 0; j < NV; ++j) {
-                unsigned t[4];
-                memcpy(t, &w[j], 16);
+                unsigned t[V / 2];
+                memcpy(t, &w[j], 2 * V);
 #pragma unroll
-                for (int k = 0; k < 4; ++k) v[j * 4 + k] = pair_up<DT>(t[k]);
+                for (int k = 0; k < V / 2; ++k) v[j * (V / 2) + k] = pair_up<DT>(t[k]);
             }
         }
     }
@@ -100,10 +100,10 @@ template <int DT, int V, int NV> struct Row {
         } else if constexpr (DT == CS2D_F32) {
             memcpy(&w, &v[j * 2], 16);
         } else {
-            unsigned t[4];
+            unsigned t[V / 2];
 #pragma unroll
-            for (int k = 0; k < 4; ++k) t[k] = pair_down<DT>(v[j * 4 + k]);
-            memcpy(&w, t, 16);
+            for (int k = 0; k < V / 2; ++k) t[k] = pair_down<DT>(v[j * (V / 2) + k]);
+            memcpy(&w, t, 2 * V);
         }
         return w;
     }
@@ -269,7 +269,7 @@ struct Tile {
 };
 
 // CTAs that an SM is to hold: the lane's values, a parameter's and the gate's, and 25 registers more
-template <int DT, int V, int NV, bool GATED> constexpr int FWD_CTAS = NV * V <= 8 ? 6 : NV * V < 16 ? 4 : GATED && (DT == CS2D_F32 || V == 1) ? 2 : 3;
+template <int DT, int V, int NV, bool GATED> constexpr int FWD_CTAS = NV * V <= 8 && V > 1 ? 6 : NV * V < 16 ? 4 : GATED && (DT == CS2D_F32 || V == 1) ? 2 : 3;
 
 template <int DT, int V, int NV, bool GATED, bool IMAGE>
 __global__ void __launch_bounds__(NT, (FWD_CTAS<DT, V, NV, GATED>)) norm_fwd(const Norm P, const Layout lay) {
@@ -353,23 +353,23 @@ __global__ void __launch_bounds__(NT, (FWD_CTAS<DT, V, NV, GATED>)) norm_fwd(con
     }
 }
 
-template <int DT, int V, int NV, bool GATED> constexpr int BWD_CTAS = NV * V <= 8 ? 4 : NV * V <= 12 && V > 1 ? 3 : 2;
+template <int DT, int V, int NV, bool GATED> constexpr int BWD_CTAS = V == 1 ? 2 : NV * V <= 8 ? 4 : NV * V <= 12 ? 3 : 2;   // single elements take registers for their addresses
 // Rows are copied to shared memory one row ahead: every lane copies the vectors that it will read itself, so nobody waits for others.
 template <int BYTES> __device__ __forceinline__ void copy_async(void *dst, const void *src) {
-    if constexpr (BYTES == 16)
-        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((unsigned)__cvta_generic_to_shared(dst)), "l"(src) : "memory");
-    else
-        asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"((unsigned)__cvta_generic_to_shared(dst)), "l"(src) : "memory");
+    const unsigned d = (unsigned)__cvta_generic_to_shared(dst);
+    if constexpr (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(d), "l"(src) : "memory");
+    else asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(d), "l"(src), "n"(BYTES) : "memory");
 }
-template <int V, int NV, bool GATED, bool IMAGE> constexpr int STAGE_BYTES = V == 1 ? 0 : NT * (16 * NV * (1 + GATED + !IMAGE) + 8);   // one row ahead, per CTA
+template <int DT, int V> constexpr int VEC_BYTES = V * (DT == CS2D_F32 ? 4 : 2);   // of an access; single 16-bit elements are not copied ahead
+template <int DT, int V, int NV, bool GATED, bool IMAGE> constexpr int STAGE_BYTES = VEC_BYTES<DT, V> < 4 ? 0 : NT * (VEC_BYTES<DT, V> * NV * (1 + GATED + !IMAGE) + 8);   // one row ahead, per CTA
 
 template <int DT, int V, int NV, bool GATED, bool IMAGE>
 __global__ void __launch_bounds__(NT, (BWD_CTAS<DT, V, NV, GATED>)) norm_bwd(const Norm P, const Layout lay) {
     using R = Row<DT, V, NV>;
     using W = typename R::W;
     using T = typename R::T;
-    constexpr bool FULL = DT == CS2D_F32, AHEAD = V > 1;
-    constexpr int H = R::H, STAGE = STAGE_BYTES<V, NV, GATED, IMAGE>;
+    constexpr bool FULL = DT == CS2D_F32, AHEAD = VEC_BYTES<DT, V> >= 4;
+    constexpr int H = R::H, VB = VEC_BYTES<DT, V>, STAGE = STAGE_BYTES<DT, V, NV, GATED, IMAGE>;
     extern __shared__ __align__(16) unsigned char smem[];
     unsigned char *tile = smem + 2 * STAGE;
     __shared__ float2 slots[2][NWARP];
@@ -378,7 +378,7 @@ __global__ void __launch_bounds__(NT, (BWD_CTAS<DT, V, NV, GATED>)) norm_bwd(con
     const float inv = 1.f / P.dim;
     const int64_t x_step = groups * P.x_is, z_step = groups * P.g_is, d_step = groups * P.dy_is;
     // the lane's vectors in a stage: stats, dy, z, x
-    auto vec_at = [&](int stage, int k, int j) { return (W *)(smem + stage * STAGE + NT * 8 + ((k * NV + j) * NT + threadIdx.x) * 16); };
+    auto vec_at = [&](int stage, int k, int j) { return (W *)(smem + stage * STAGE + NT * 8 + ((k * NV + j) * NT + threadIdx.x) * VB); };
     auto stat_at = [&](int stage) { return (float2 *)(smem + stage * STAGE + threadIdx.x * 8); };
     // the row that is copied next
     const T *xp = nullptr, *dp = nullptr, *zp = nullptr;
@@ -397,14 +397,14 @@ __global__ void __launch_bounds__(NT, (BWD_CTAS<DT, V, NV, GATED>)) norm_bwd(con
         t_next += gridDim.x;
     };
     auto ahead = [&](int stage) {
-        if (p_next + g < n_next) {
+        if constexpr (AHEAD) if (p_next + g < n_next) {
             copy_async<8>(stat_at(stage), sp);
 #pragma unroll
             for (int j = 0; j < NV; ++j) {
                 if (j * TL + l >= nvec) continue;
-                copy_async<16>(vec_at(stage, 0, j), dp + j * TL * V);
-                if (GATED) copy_async<16>(vec_at(stage, 1, j), zp + j * TL * V);
-                if (!IMAGE) copy_async<16>(vec_at(stage, 1 + GATED, j), xp + j * TL * V);
+                copy_async<VB>(vec_at(stage, 0, j), dp + j * TL * V);
+                if (GATED) copy_async<VB>(vec_at(stage, 1, j), zp + j * TL * V);
+                if (!IMAGE) copy_async<VB>(vec_at(stage, 1 + GATED, j), xp + j * TL * V);
             }
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
@@ -556,10 +556,10 @@ template <auto KERNEL> cudaError_t start(const Norm &P, const Layout &l, size_t 
 template <bool BWD, int DT, int V, int NV> cudaError_t go(const Norm &P, const Layout &l, size_t smem, cudaStream_t st) {
     const bool image = l.image;
     if constexpr (BWD) {
-        if (P.gate) return image ? start<norm_bwd<DT, V, NV, true, true>>(P, l, smem + 2 * STAGE_BYTES<V, NV, true, true>, st)
-                                 : start<norm_bwd<DT, V, NV, true, false>>(P, l, smem + 2 * STAGE_BYTES<V, NV, true, false>, st);
-        return image ? start<norm_bwd<DT, V, NV, false, true>>(P, l, smem + 2 * STAGE_BYTES<V, NV, false, true>, st)
-                     : start<norm_bwd<DT, V, NV, false, false>>(P, l, smem + 2 * STAGE_BYTES<V, NV, false, false>, st);
+        if (P.gate) return image ? start<norm_bwd<DT, V, NV, true, true>>(P, l, smem + 2 * STAGE_BYTES<DT, V, NV, true, true>, st)
+                                 : start<norm_bwd<DT, V, NV, true, false>>(P, l, smem + 2 * STAGE_BYTES<DT, V, NV, true, false>, st);
+        return image ? start<norm_bwd<DT, V, NV, false, true>>(P, l, smem + 2 * STAGE_BYTES<DT, V, NV, false, true>, st)
+                     : start<norm_bwd<DT, V, NV, false, false>>(P, l, smem + 2 * STAGE_BYTES<DT, V, NV, false, false>, st);
     } else {
         if (P.gate) return image ? start<norm_fwd<DT, V, NV, true, true>>(P, l, smem, st) : start<norm_fwd<DT, V, NV, true, false>>(P, l, smem, st);
         return image ? start<norm_fwd<DT, V, NV, false, true>>(P, l, smem, st) : start<norm_fwd<DT, V, NV, false, false>>(P, l, smem, st);
@@ -570,14 +570,20 @@ template <bool BWD, int DT> cudaError_t launch(const Norm &P, const Layout &l, i
     if (v == V) switch (nv) {
             case 1: return go<BWD, DT, V, 1>(P, l, smem, st);
             case 2: return go<BWD, DT, V, 2>(P, l, smem, st);
-            case 3: if constexpr (BWD) return P.gate || l.image ? cudaErrorInvalidValue : start<norm_bwd<DT, V, 3, false, false>>(P, l, smem + 2 * STAGE_BYTES<V, 3, false, false>, st);
+            case 3: if constexpr (BWD) return P.gate || l.image ? cudaErrorInvalidValue : start<norm_bwd<DT, V, 3, false, false>>(P, l, smem + 2 * STAGE_BYTES<DT, V, 3, false, false>, st);
                     else return go<BWD, DT, V, 3>(P, l, smem, st);
             case 6: if constexpr (DT == CS2D_F32 && !BWD) return go<BWD, DT, V, 6>(P, l, smem, st);
         }
+    else if (v == 2) switch (nv) {
+            case 2: if constexpr (DT != CS2D_F32) return go<BWD, DT, 2, 2>(P, l, smem, st);
+            case 4: if constexpr (DT != CS2D_F32) return go<BWD, DT, 2, 4>(P, l, smem, st);
+            case 6: if constexpr (DT != CS2D_F32) return go<BWD, DT, 2, 6>(P, l, smem, st);
+        }
     else switch (nv) {
             case 4: return go<BWD, DT, 1, 4>(P, l, smem, st);
+            case 6: return go<BWD, DT, 1, 6>(P, l, smem, st);
+            case 8: return go<BWD, DT, 1, 8>(P, l, smem, st);
             case 12: return go<BWD, DT, 1, 12>(P, l, smem, st);
-            case 24: return go<BWD, DT, 1, 24>(P, l, smem, st);
         }
     return cudaErrorInvalidValue;
 }

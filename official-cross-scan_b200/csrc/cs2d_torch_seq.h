@@ -281,12 +281,13 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
         if (p.x_cs == 1) {
             dx = at::empty(a.x.sizes(), a.x.options());
         } else {   // a channel-major image: its gradient is one too
-            std::vector<int64_t> sizes(a.x.sizes().begin(), a.x.sizes().end());
-            const int64_t split = a.x.dim() >= 3 ? 1 : 0;
-            std::vector<int64_t> dense(sizes.begin(), sizes.begin() + split);
-            dense.push_back(p.dim);
-            dense.insert(dense.end(), sizes.begin() + split, sizes.end() - 1);
-            dx = at::empty(dense, a.x.options()).movedim(split, -1);
+            const int64_t n = a.x.dim();
+            c10::SmallVector<int64_t, 6> strides(n);
+            strides[n - 1] = p.inner;
+            int64_t run = 1;
+            for (int64_t d = n - 2; d >= (n >= 3 ? 1 : 0); --d) { strides[d] = run; run *= a.x.size(d); }
+            if (n >= 3) strides[0] = p.inner * p.dim;
+            dx = at::empty_strided(a.x.sizes(), strides, a.x.options());
             is = 1; cs = p.inner;
         }
         const size_t nbytes = cs2d_norm_bwd_scratch_bytes(&p);
