@@ -27,7 +27,6 @@ namespace nm {
 
 constexpr int NT = 256;       // threads of a CTA
 constexpr int NWARP = NT / 32;
-constexpr int MAXE = 24;      // channels of a lane, at most
 
 struct Layout {
     int T, P, pitch;             // lanes of a row; rows of a tile; images: bytes between them in shared memory

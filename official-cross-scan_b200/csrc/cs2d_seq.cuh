@@ -5,10 +5,8 @@
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
-#include <cstring>
-#include <type_traits>
-
 #include <cstdint>
+#include <cstring>
 
 #include "../../include/cs2d.h"
 #include "cs2d_status.h"
@@ -30,9 +28,9 @@ struct GScan {
     int *status;
 };
 enum { SEQ_NONE = -1, SEQ_OUTSIDE = -2 };
-enum { GS_CHUNKS = 0, GS_WORDS = 1, GS_ELEMENTS = 2 };   // 16 bytes, a lane's two channels, one channel at a time
+enum { GS_CHUNKS = 0, GS_WORDS = 1, GS_ELEMENTS = 2 };   // 16 bytes, 4 bytes, one 16-bit channel at a time
 
-constexpr int GS_CK = 32;       // rows between two checkpoints; the backward's tiles are multiples of it
+constexpr int GS_CK = 32;       // rows between two checkpoints: a multiple of the rows of a warp in the backward
 
 cudaError_t launch_gscan_map(const GScan &P, cudaStream_t st);
 cudaError_t launch_gscan_fwd(const GScan &P, int dt, cudaStream_t st);
@@ -74,30 +72,12 @@ template <> struct Elem<CS2D_BF16> {
     static __device__ __forceinline__ T down(float v) { return __float2bfloat16_rn(v); }
 };
 
-// V consecutive elements as the word that they are loaded and stored as
+// The word that so many bytes are loaded and stored as
 template <int BYTES> struct WordOf;
 template <> struct WordOf<2> { using W = uint16_t; };
 template <> struct WordOf<4> { using W = uint32_t; };
 template <> struct WordOf<8> { using W = uint2; };
 template <> struct WordOf<16> { using W = uint4; };
-template <int DT, int V> struct Pack {
-    using T = typename Elem<DT>::T;
-    using W = typename WordOf<sizeof(T) * V>::W;
-    static __device__ __forceinline__ void up(W w, float (&v)[V]) {
-        T t[V];
-        memcpy(t, &w, sizeof(w));
-#pragma unroll
-        for (int k = 0; k < V; ++k) v[k] = Elem<DT>::up(t[k]);
-    }
-    static __device__ __forceinline__ W down(const float (&v)[V]) {
-        T t[V];
-        W w;
-#pragma unroll
-        for (int k = 0; k < V; ++k) t[k] = Elem<DT>::down(v[k]);
-        memcpy(&w, t, sizeof(w));
-        return w;
-    }
-};
 
 // ---- the gate: its factor a and c = 1 - a, each to a few units of its own last place ---------------------------
 // FULL: for fp32 inputs; 16-bit ones take the hardware's exponential and reciprocal (denormals flushed).

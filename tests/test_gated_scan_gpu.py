@@ -317,3 +317,23 @@ def test_refusals():
                       ((v.clone().requires_grad_(True), v, h), "no gradient"), ((v, v, h[:1]), "shape of u")]:
         with pytest.raises(RuntimeError, match=msg):
             cs2d.gated_scan_step(*args)
+
+
+def test_more_elements_than_32_bits_count():
+    """2 x 1100000 x 1024 bf16 elements: a gate of zero passes every input on, one of one adds up what a counting input brings."""
+    if torch.cuda.mem_get_info()[0] < 40 << 30:
+        pytest.skip("needs 40 GB")
+    u = torch.empty(2, 1100000, 1024, dtype=BF16, device="cuda")
+    for b in range(2):
+        for i in range(0, u.shape[1], 100000):
+            u[b, i:i + 100000].normal_()
+    with torch.no_grad():
+        y, last = cs2d.gated_scan_1d(u, torch.zeros(1, 1, 1024, dtype=BF16, device="cuda").expand_as(u), None, form="direct", weighted=False)
+        assert torch.equal(y, u) and torch.equal(last, u[:, -1].float())
+        del y
+        n = cs2d.layer_norm(u, eps=1e-5)
+        for at in (0, 1048575, 1048576, 1099999):
+            for b in range(2):
+                row = u[b, at].double()
+                want = (row - row.mean()) / (row.var(unbiased=False) + 1e-5).sqrt()
+                assert float((n[b, at].double() - want).abs().max()) <= 4 * (R.half_step(BF16) + 1e-5) * float(want.abs().max())
