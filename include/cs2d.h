@@ -271,7 +271,8 @@ int cs2d_bwd_noalloc(const cs2d_problem *p, const void *dout, int64_t dout_bs, i
  * (device, n_seq + 1 ascending int32, or int64 where offsets64 is set) cuts the rows into n_seq sequences
  * [offsets[s], offsets[s+1]) with a state each; a sequence may be empty (its h0 passes through).  Rows of no sequence
  * are not read; y, du and dgate are zero there.  Offsets that do not ascend or leave the tensor set bit 3 of the status
- * word; the outputs are then invalid, nothing outside of them is touched.
+ * word; the outputs are then invalid, nothing outside of them is touched.  At most 2^30 channels and rows, fewer than 2^30
+ * sequences: CS2D_ERR_UNSUPPORTED otherwise.
  */
 typedef enum { CS2D_GATE_SIGMOID = 0, CS2D_GATE_LOG = 1, CS2D_GATE_DIRECT = 2 } cs2d_gate_form;
 typedef struct {
@@ -317,6 +318,7 @@ int cs2d_gscan_step(const cs2d_gscan *p, void *y, int64_t y_bs, float *h, int64_
  * (channel-major images) must be 1.  gate: channel stride 1, or NULL.  weight, bias (dim) of param_dtype (fp32 or the
  * input type), dense, or NULL (ones, zeros).  y (outer, inner, dim) of io_dtype, dense.  stats (outer * inner, 2) fp32, 8-byte aligned, receives mean
  * and 1 / sqrt(var + eps) for the backward, or NULL.  Sums and statistics are fp32, the variance that of the centred values.
+ * At most 2^31 rows and 2^29 channels: CS2D_ERR_UNSUPPORTED otherwise.
  */
 typedef struct {
     int32_t dim, io_dtype, param_dtype;

@@ -13,9 +13,12 @@ static int validate(const cs2d_gscan *p, bool step) {
     if (p->form < CS2D_GATE_SIGMOID || p->form > CS2D_GATE_DIRECT) return fail(CS2D_ERR_INVALID, "unknown form of the gate: %d", p->form);
     if (!p->u || !p->gate) return fail(CS2D_ERR_INVALID, "u and gate must be given");
     if (step) return CS2D_OK;
+    // (the kernels count channels, tokens and sequences in 32 bits, up to a unit's, a cluster's or a search interval's end behind the last one)
     if (p->length > (1 << 30)) return fail(CS2D_ERR_UNSUPPORTED, "more than 2^30 tokens in a row");
+    if (p->dim > (1 << 30)) return fail(CS2D_ERR_UNSUPPORTED, "more than 2^30 channels");
     if (p->offsets && p->batch != 1) return fail(CS2D_ERR_INVALID, "with offsets the batch is 1");
     if (p->offsets && p->n_seq < 0) return fail(CS2D_ERR_INVALID, "n_seq must not be negative");
+    if (p->offsets && p->n_seq >= (1 << 30)) return fail(CS2D_ERR_UNSUPPORTED, "2^30 sequences or more");
     return CS2D_OK;
 }
 // Every row starts on a multiple of `bytes`, and so does what is behind its last channel.
@@ -58,6 +61,7 @@ static int validate(const cs2d_norm *p) {
     if (p->io_dtype < CS2D_F32 || p->io_dtype > CS2D_BF16) return fail(CS2D_ERR_INVALID, "input type must be float32, float16 or bfloat16");
     if (p->param_dtype != CS2D_F32 && p->param_dtype != p->io_dtype)
         return fail(CS2D_ERR_INVALID, "weight and bias must be float32 or of the input type");
+    if (p->dim > (1 << 29)) return fail(CS2D_ERR_UNSUPPORTED, "more than 2^29 channels");   // 2 dim and what a warp's step leads to fit 32 bits
     if (!p->x) return fail(CS2D_ERR_INVALID, "x must be given");
     if (p->x_cs != 1 && p->x_is != 1) return fail(CS2D_ERR_INVALID, "x must have stride 1 along its channels or its rows");
     if (p->outer > ((int64_t)1 << 31) / p->inner) return fail(CS2D_ERR_UNSUPPORTED, "more than 2^31 rows");

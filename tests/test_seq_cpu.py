@@ -92,3 +92,17 @@ def test_norm_validation_happens_before_any_cuda_call(over, msg):
         setattr(p, k, v)
     assert L.cs2d_norm_bwd_scratch_bytes(ctypes.byref(p)) == 0 and msg in L.cs2d_last_error().decode()
     assert L.cs2d_norm_fwd(ctypes.byref(p), ctypes.c_void_p(256), None, None) < 0
+
+
+def test_counts_that_the_kernels_cannot_hold_are_refused():
+    """Channels, rows and sequences are counted in 32 bits on the GPU: what such a count would pass is refused before any CUDA call."""
+    L = _lib_with_types()
+    scan = lambda **over: L.cs2d_gscan_saved_bytes(ctypes.byref(_gscan(**over)), 0)
+    assert scan(dim=1 << 30) and scan(batch=1, length=1 << 30) and scan(batch=1, offsets=256, n_seq=(1 << 30) - 1)
+    for over, msg in ((dict(dim=(1 << 30) + 1), "channels"), (dict(dim=(1 << 31) - 1), "channels"), (dict(batch=1, length=(1 << 30) + 1), "tokens"),
+                      (dict(batch=1, offsets=256, n_seq=1 << 30), "sequences"), (dict(batch=1, offsets=256, n_seq=(1 << 31) - 1), "sequences")):
+        assert scan(**over) == 0 and msg in L.cs2d_last_error().decode(), over
+    norm = lambda dim: L.cs2d_norm_bwd_scratch_bytes(ctypes.byref(NormP(dim=dim, io_dtype=_lib.BF16, param_dtype=_lib.F32, eps=1e-5, outer=1, inner=1, x=256, x_cs=1)))
+    assert norm(1 << 29)
+    for dim in ((1 << 29) + 1, (1 << 31) - 1):
+        assert norm(dim) == 0 and "channels" in L.cs2d_last_error().decode()
