@@ -65,6 +65,8 @@ class SS2D(nn.Module):
     channel-major image as it lies and rounds once; same parameters and state dict.
     """
 
+    fused_norm = False   # of modules pickled before the option existed
+
     def __init__(self, d_model: int, d_state: int = 16, expand: int = 2, dt_rank: int | None = None, d_conv: int = 3,
                  directions: int = 4, device=None, fused_norm: bool = False):
         super().__init__()

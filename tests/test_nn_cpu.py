@@ -32,3 +32,17 @@ def test_block_shapes_and_projection_layout():
     assert seen["B"].shape == seen["C"].shape == (2, 4, 4, 6, 10)
     assert seen["B"].stride(-1) == 1 and seen["B"].data_ptr() != seen["C"].data_ptr()
     assert seen["B"]._base is not None and seen["B"]._base is seen["C"]._base      # views of one tensor
+
+
+def test_a_block_that_was_pickled_before_the_option_existed():
+    """A whole module saved by an earlier version has no fused_norm among its attributes: it runs as it did."""
+    import io
+    m = SS2D(d_model=8, d_state=2)
+    del m.__dict__["fused_norm"]
+    buf = io.BytesIO()
+    torch.save(m, buf)
+    buf.seek(0)
+    old = torch.load(buf, weights_only=False)
+    assert old.fused_norm is False
+    old._scan = lambda u, delta, A, B, C, w, D, dt_bias: u
+    assert old(torch.randn(1, 3, 4, 8)).shape == (1, 3, 4, 8)
