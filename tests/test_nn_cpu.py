@@ -37,6 +37,7 @@ def test_block_shapes_and_projection_layout():
 def test_a_block_that_was_pickled_before_the_option_existed():
     """A whole module saved by an earlier version has no fused_norm among its attributes: it runs as it did."""
     import io
+    from cs2d.nn import SS2D
     m = SS2D(d_model=8, d_state=2)
     del m.__dict__["fused_norm"]
     buf = io.BytesIO()
