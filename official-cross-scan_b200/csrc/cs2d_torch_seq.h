@@ -157,6 +157,7 @@ Tensor py_gated_step(const Tensor &u, const Tensor &gate, const Tensor &h, int64
     CS2D_CHECK(h.scalar_type() == at::kFloat && h.sizes() == u.sizes(), "h must be float32 with the shape of u");
     CS2D_CHECK((h.stride(1) == 1 || h.size(1) <= 1) && (h.size(0) <= 1 || h.stride(0) >= h.size(1)),
                "h is updated in place: its rows must be contiguous and must not overlap");
+    CS2D_CHECK(!h.is_inference() || c10::InferenceMode::is_enabled(), "h is an inference tensor: outside inference mode it cannot be updated in place");
     CS2D_CHECK(u.size(0) <= INT32_MAX && u.size(1) <= INT32_MAX, "u is too large");
     const c10::cuda::CUDAGuard guard(u.device());
     const Tensor ur = rows_of(u), gr = rows_of(gate);

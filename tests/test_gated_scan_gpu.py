@@ -337,3 +337,15 @@ def test_more_elements_than_32_bits_count():
                 row = u[b, at].double()
                 want = (row - row.mean()) / (row.var(unbiased=False) + 1e-5).sqrt()
                 assert float((n[b, at].double() - want).abs().max()) <= 4 * (R.half_step(BF16) + 1e-5) * float(want.abs().max())
+
+
+def test_a_state_that_may_not_be_written_stays_as_it_is():
+    """An inference tensor outside inference mode: refused, as torch refuses it, before anything is written."""
+    u = torch.randn(2, 8, device="cuda")
+    with torch.inference_mode():
+        h = torch.ones(2, 8, device="cuda")
+        before = cs2d.gated_scan_step(u, u, h).clone()
+        kept = h.clone()
+    with pytest.raises(RuntimeError, match="inference"):
+        cs2d.gated_scan_step(u, u, h)
+    assert torch.equal(h, kept) and torch.isfinite(before).all()
