@@ -17,6 +17,6 @@ def layer_norm(x, weight=None, bias=None, gate=None, eps=1e-5):
     ``x``: ``(..., dim)``, float32, float16 or bfloat16.  ``weight``, ``bias``: ``(dim,)``, float32 or the dtype of ``x``, or None.  ``gate``:
     the shape and dtype of ``x``, or None for no gate.  Other strides than those of token rows and channel-major images cost a copy.
     The gradients of ``weight`` and ``bias`` are sums over the rows in float32 and a fixed order: every result comes out
-    with the same bits on every run.
+    with the same bits on every run.  No forward-mode derivative: an input with a tangent is refused.
     """
     return _lib.native().layer_norm(x, weight, bias, gate, float(eps))

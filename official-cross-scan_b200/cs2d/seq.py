@@ -44,6 +44,7 @@ def gated_scan_1d(u, gate, h0=None, offsets=None, form="sigmoid", weighted=True)
     Offsets that do not ascend or leave the tensor are found on the GPU and reported by ``cs2d.device_status()``.
 
     Gradients go to ``u``, ``gate`` and ``h0``, from ``y`` and ``h_last``.  When nothing can ask for one, no state is kept.
+    No forward-mode derivative: an input with a tangent is refused, here and in ``gated_scan_step``.
     """
     return _lib.native().gated_scan(u, gate, h0, offsets, _form(form), bool(weighted))
 

@@ -17,6 +17,11 @@ void no_stale_leaves(std::initializer_list<const Tensor *> inputs) {
 void once_differentiable(const char *what) {
     CS2D_CHECK(!at::GradMode::is_enabled(), what, " has no second derivative: call the backward without create_graph");
 }
+// Forward-mode differentiation: a tangent would be lost without a word where nothing wants a gradient.
+void no_tangents(std::initializer_list<const Tensor *> inputs, const char *what) {
+    if (!c10::AutogradState::get_tls_state().get_fw_grad_mode()) return;
+    for (const Tensor *t : inputs) CS2D_CHECK(!given(*t) || !t->_fw_grad(0).defined(), what, " has no forward-mode derivative");
+}
 int64_t step_of(const Tensor &t, int64_t d) { return t.size(d) > 1 ? t.stride(d) : 0; }
 Tensor rows_of(const Tensor &t) { return t.stride(-1) == 1 || t.size(-1) <= 1 ? t : t.contiguous(); }
 void same_place(const Tensor &t, const Tensor &like, const char *name) {
@@ -133,8 +138,9 @@ struct GatedScan : torch::autograd::Function<GatedScan> {
 };
 
 std::tuple<Tensor, Tensor> py_gated_scan(const Tensor &u, const Tensor &gate, const OptT &h0, const OptT &offsets, int64_t form, bool weighted) {
-    if (at::GradMode::is_enabled() && (wants_grad(u) || wants_grad(gate) || wants_grad(opt(h0)))) {
-        const Tensor h = opt(h0);
+    const Tensor h = opt(h0);
+    no_tangents({&u, &gate, &h}, "gated_scan_1d");
+    if (at::GradMode::is_enabled() && (wants_grad(u) || wants_grad(gate) || wants_grad(h))) {
         no_stale_leaves({&u, &gate, &h});
         const variable_list r = GatedScan::apply(u, gate, h0, offsets, form, weighted);
         return {r[0], r[1]};
@@ -147,6 +153,7 @@ std::tuple<Tensor, Tensor> py_gated_scan(const Tensor &u, const Tensor &gate, co
 Tensor py_gated_step(const Tensor &u, const Tensor &gate, const Tensor &h, int64_t form, bool weighted) {
     CS2D_CHECK(!(at::GradMode::is_enabled() && (wants_grad(u) || wants_grad(gate) || wants_grad(h))),
                "gated_scan_step has no gradient: call it under torch.no_grad(), or gated_scan_1d on one token");
+    no_tangents({&u, &gate, &h}, "gated_scan_step");
     at::NoGradGuard no_grad;
     CS2D_CHECK(u.is_cuda(), "u must be a CUDA tensor");
     CS2D_CHECK(dtype_code(u.scalar_type()) >= 0, "gated_scan_step not implemented for input type '", u.scalar_type(), "'");
@@ -311,6 +318,7 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
 
 Tensor py_layer_norm(const Tensor &x, const OptT &weight, const OptT &bias, const OptT &gate, double eps) {
     const Tensor w = opt(weight), b = opt(bias), z = opt(gate);
+    no_tangents({&x, &w, &b, &z}, "layer_norm");
     if (at::GradMode::is_enabled() && (wants_grad(x) || wants_grad(w) || wants_grad(b) || wants_grad(z))) {
         no_stale_leaves({&x, &w, &b, &z});
         return LayerNorm::apply(x, weight, bias, gate, eps);

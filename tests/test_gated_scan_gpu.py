@@ -349,3 +349,27 @@ def test_a_state_that_may_not_be_written_stays_as_it_is():
     with pytest.raises(RuntimeError, match="inference"):
         cs2d.gated_scan_step(u, u, h)
     assert torch.equal(h, kept) and torch.isfinite(before).all()
+
+
+def test_tangents_are_refused_not_lost():
+    """Forward-mode differentiation is not implemented: an input with a tangent raises, whether it wants a gradient or not."""
+    import torch.autograd.forward_ad as fw
+    u, h, off = torch.randn(2, 5, 8, device="cuda"), torch.randn(2, 8, device="cuda"), torch.tensor([0, 2, 5], device="cuda")
+    w = torch.ones(8, device="cuda")
+    for needs in (False, True):
+        with fw.dual_level():
+            dual = lambda t: fw.make_dual(t.clone().requires_grad_(needs), torch.ones_like(t))
+            calls = [lambda: cs2d.gated_scan_1d(dual(u), u, h), lambda: cs2d.gated_scan_1d(u, dual(u), h), lambda: cs2d.gated_scan_1d(u, u, dual(h)),
+                     lambda: cs2d.gated_scan_1d(u[0], dual(u[0]), None, off), lambda: cs2d.layer_norm(dual(u)), lambda: cs2d.layer_norm(u, dual(w)),
+                     lambda: cs2d.layer_norm(u, w, dual(w)), lambda: cs2d.layer_norm(u, w, None, dual(u))]
+            for i, call in enumerate(calls):
+                with pytest.raises(RuntimeError, match="forward-mode"):
+                    call()
+                with pytest.raises(RuntimeError, match="forward-mode"), torch.no_grad():
+                    call()
+            with torch.no_grad():
+                for args in ((dual(u[:, 0]), u[:, 0], h), (u[:, 0], dual(u[:, 0]), h), (u[:, 0], u[:, 0], dual(h))):
+                    with pytest.raises(RuntimeError, match="forward-mode"):
+                        cs2d.gated_scan_step(*args)
+    with torch.no_grad():
+        assert cs2d.layer_norm(u).shape == u.shape and cs2d.gated_scan_step(u[:, 0], u[:, 0], h).shape == h.shape
