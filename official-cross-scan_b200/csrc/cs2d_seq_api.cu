@@ -73,7 +73,14 @@ static Norm fill(const cs2d_norm *p) {
     d.x = p->x; d.x_os = p->x_os; d.x_is = p->x_is; d.x_cs = p->x_cs;
     d.gate = p->gate; d.g_os = p->g_os; d.g_is = p->g_is;
     d.weight = p->weight; d.bias = p->bias;
-    if (d.x_os == d.inner * d.x_is && (!d.gate || d.g_os == d.inner * d.g_is)) d.inner = d.rows;   // one run of rows
+    // One run of rows: the outer index goes on where the inner one ends, or is the only one (whose stride then is that of the rows).
+    if (p->inner == 1 && (d.x_cs == 1 || d.x_os == 1)) {
+        d.inner = d.rows;
+        d.x_is = d.x_os;
+        d.g_is = d.g_os;
+    } else if (d.x_os == d.inner * d.x_is && (!d.gate || d.g_os == d.inner * d.g_is)) {
+        d.inner = d.rows;
+    }
     d.parts = norm_parts(d, p->io_dtype);
     return d;
 }
@@ -154,8 +161,14 @@ int cs2d_norm_bwd(const cs2d_norm *p, const void *dy, int64_t dy_os, int64_t dy_
     if (dx_cs != 1 && dx_is != 1) return fail(CS2D_ERR_INVALID, "dx must have stride 1 along its channels or its rows");
     Norm d = fill(p);
     d.dy = dy; d.dy_os = dy_os; d.dy_is = dy_is; d.stats = const_cast<float *>(stats); d.part = (float *)scratch;
-    if (d.inner != p->inner && (dy_os != p->inner * dy_is || dx_os != p->inner * dx_is)) d.inner = p->inner;
-    d.dx = dx; d.dx_os = dx_os; d.dx_is = dx_is; d.dx_cs = dx_cs; d.dgate = dgate; d.dweight = dweight; d.dbias = dbias;
+    d.dx = dx; d.dx_os = dx_os; d.dx_is = dx_is; d.dx_cs = dx_cs;
+    if (p->inner == 1 && d.inner != 1 && (dx_cs == 1 || dx_os == 1)) {
+        d.dy_is = dy_os;
+        d.dx_is = dx_os;
+    } else if (d.inner != p->inner && (dy_os != p->inner * dy_is || dx_os != p->inner * dx_is)) {
+        d.inner = p->inner;
+    }
+    d.dgate = dgate; d.dweight = dweight; d.dbias = dbias;
     int n = 0;
     const cudaError_t e = launch_norm_bwd(d, p->io_dtype, static_cast<cudaStream_t>(stream), &n);
     return launched(e, n);

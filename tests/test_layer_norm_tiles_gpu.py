@@ -103,3 +103,34 @@ def test_more_elements_than_32_bits_count_backward(image):
     # D / 32 + 32 units of the largest of its row (below 8)
     assert ((dw.double() - total).abs() <= (B * L / 1024 + 64) * U * size + B * L * 8 * (D / 32 + 32) * U).all()
     assert (total[0] < -0.5 * B * L) and (total[-1] > 0.5 * B * L)
+
+
+@pytest.mark.parametrize("dtype", (F32, F16, BF16))
+@pytest.mark.parametrize("dim", (51, 192, 768))
+def test_an_axis_of_one_between_rows_and_channels(dim, dtype):
+    """(B, 1, dim), as tokens that are decoded together or maps of one position have it, is (B, dim): the same kernels, so the same bits."""
+    d = inputs((6001,), dim, dtype, True, seed=dim)
+    plain = run(d)
+    for shape in ((6001, 1, dim), (6001, 1, 1, dim)):
+        e = {k: v.reshape(shape) if v.dim() > 1 else v for k, v in d.items()}
+        got = run(e)
+        for k, v in got.items():
+            assert torch.equal(v, plain[k].reshape(v.shape)), (k, shape)
+
+
+def test_an_axis_of_one_with_strides_of_each_their_own():
+    """x, gate and dy are columns of wider tensors, of one width each; the same for images of one position and for one row."""
+    B, D = 700, 96
+    d = inputs((B, 1), 3 * D, BF16, True)
+    e = {"x": d["x"][..., D:2 * D], "gate": torch.cat([d["gate"], d["gate"]], -1)[..., 8:D + 8], "dy": d["dy"][:, :, :D].contiguous(),
+         "weight": d["weight"][:D], "bias": d["bias"][:D]}
+    check(e, run(e))
+    e["dy"] = d["dy"][..., :D]
+    check(e, run(e))
+    e["x"] = d["x"][:, 0, :D].t().contiguous().t()[:, None]        # channels apart: a copy
+    check(e, run(e))
+    one = {k: v[:1] if v.dim() > 1 else v for k, v in e.items()}
+    check(one, run(one))
+    image = dict(e, x=torch.randn(B, D, 1, 1, device="cuda").to(BF16).permute(0, 2, 3, 1))
+    image.update(gate=e["gate"][:, None], dy=e["dy"][:, None])
+    check(image, run(image))
