@@ -16,6 +16,7 @@
 
 #include <cooperative_groups.h>
 
+#include <atomic>
 #include <cstring>
 
 #include "cs2d_seq.cuh"
@@ -404,19 +405,22 @@ inline void configure(cudaLaunchConfig_t &cfg, cudaLaunchAttribute *attr, int64_
 }
 // Launches KERNEL with its rows split as they should be; rows: of a warp's tile.
 template <auto KERNEL> cudaError_t start(GScan &P, int G, int rows, size_t smem, cudaStream_t st) {
-    static int at_once[64][MAXC + 1] = {};   // per device and cluster size: clusters that fit the GPU at a time
+    // Per device and cluster size: clusters that fit the GPU at a time.  The entry of size one is written last: the others are there.  Threads that
+    // come at the same time write the same numbers.
+    static std::atomic<int> at_once[64][MAXC + 1] = {};
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
     if (e != cudaSuccess || dev < 0 || dev >= 64) return e != cudaSuccess ? e : cudaErrorInvalidDevice;
     cudaLaunchConfig_t cfg;
     cudaLaunchAttribute attr[1];
-    if (!at_once[dev][1]) {
+    if (!at_once[dev][1].load(std::memory_order_acquire)) {
         if ((e = cudaFuncSetAttribute(KERNEL, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem)) != cudaSuccess) return e;
         if ((e = cudaFuncSetAttribute(KERNEL, cudaFuncAttributeNonPortableClusterSizeAllowed, 1)) != cudaSuccess) return e;
         for (int C = MAXC; C >= 1; --C) {
             configure(cfg, attr, C, C, smem, st);
-            if (C == 1) at_once[dev][C] = 1;
-            else if (cudaOccupancyMaxActiveClusters(&at_once[dev][C], KERNEL, &cfg) != cudaSuccess) at_once[dev][C] = 0;
+            int n = 1;
+            if (C > 1 && cudaOccupancyMaxActiveClusters(&n, KERNEL, &cfg) != cudaSuccess) n = 0;
+            at_once[dev][C].store(n, std::memory_order_release);
         }
         cudaGetLastError();   // (a size that the device does not have)
     }
@@ -428,7 +432,7 @@ template <auto KERNEL> cudaError_t start(GScan &P, int G, int rows, size_t smem,
     // The largest cluster of which all fit the GPU at once: a second round would take as long as the first (24 units: 26 clusters of 10
     // fit, B1 L67200 D384 70 + 115 us; 21 of 12, 90 + 148 us; 33 of 8, 78 + 129 us).
     for (int C = (int)(tiles < MAXC ? tiles : MAXC); C > 1 && s.C == 1; --C)
-        if (at_once[dev][C] >= ctas) s.C = C;
+        if (at_once[dev][C].load(std::memory_order_relaxed) >= ctas) s.C = C;
     s.grid = ctas * s.C;
     configure(cfg, attr, s.grid, s.C, smem, st);
     return cudaLaunchKernelEx(&cfg, KERNEL, (const GScan)P, (const int)s.wt, (const int)s.C);

@@ -17,6 +17,7 @@
 // 123 (48 %); B16 D384 128x128 bf16 gated image 147 (63 %) and 328 (47 %).
 #pragma once
 
+#include <atomic>
 #include <cstring>
 
 #include "cs2d_seq.cuh"
@@ -539,7 +540,7 @@ __global__ void __launch_bounds__(NT, (BWD_CTAS<DT, V, NV, GATED>)) norm_bwd(con
 
 // ---- launches ----------------------------------------------------------------------------------------------------
 template <auto KERNEL> cudaError_t start(const Norm &P, const Layout &l, size_t smem, cudaStream_t st) {
-    static bool done[64] = {};   // per device
+    static std::atomic<bool> done[64] = {};   // per device; threads that come at the same time set the same attribute
     const size_t acc = (size_t)8 * P.dim;   // the backward's sums, in the place of all else
     if (P.dy && smem < acc) smem = acc;
     int dev = 0;
