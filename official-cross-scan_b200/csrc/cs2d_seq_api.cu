@@ -50,7 +50,10 @@ static int fill(GScan &d, const cs2d_gscan *p, void *saved) {
     return CS2D_OK;
 }
 static int launched(cudaError_t e, int n) {
-    if (e != cudaSuccess) return fail(CS2D_ERR_CUDA, "launch failed: %s", cudaGetErrorString(e));
+    if (e != cudaSuccess) {
+        cudaGetLastError();   // reported here: the next launch that asks for the last error finds none
+        return fail(CS2D_ERR_CUDA, "launch failed: %s", cudaGetErrorString(e));
+    }
     count_launches(n);
     return CS2D_OK;
 }

@@ -159,3 +159,35 @@ def test_first_calls_from_several_threads():
     """)
     r = subprocess.run([sys.executable, "-c", code], cwd=ROOT, capture_output=True, text=True, timeout=300)
     assert r.returncode == 0 and r.stdout.split() == ["True", "0"], r.stdout + r.stderr
+
+
+def test_a_launch_that_failed_is_not_reported_twice():
+    """In a process of its own: a recording that something else has made invalid refuses the scan's launch; the next call, on a good stream, runs."""
+    import subprocess
+    import sys
+    import textwrap
+    from conftest import ROOT
+    code = textwrap.dedent("""
+        import sys, torch
+        sys.path.insert(0, "official-cross-scan_b200")
+        import cs2d
+        u, x = torch.randn(1, 300, 64, device="cuda"), torch.randn(5, 64, device="cuda")
+        want = cs2d.layer_norm(x), cs2d.gated_scan_1d(u, u)[0]
+        torch.cuda.synchronize()
+        try:
+            with torch.cuda.graph(torch.cuda.CUDAGraph()):
+                try:
+                    torch.cuda.synchronize()            # not allowed while recording
+                except RuntimeError:
+                    pass
+                try:
+                    cs2d.gated_scan_1d(u, u)
+                    print("launched")
+                except RuntimeError as e:
+                    print("refused" if "launch failed" in str(e) else e)
+        except RuntimeError:
+            print("invalid")
+        print(torch.equal(cs2d.layer_norm(x), want[0]), torch.equal(cs2d.gated_scan_1d(u, u)[0], want[1]))
+    """)
+    r = subprocess.run([sys.executable, "-c", code], cwd=ROOT, capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and r.stdout.split() == ["refused", "invalid", "True", "True"], r.stdout + r.stderr
