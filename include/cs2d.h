@@ -269,9 +269,10 @@ int cs2d_bwd_noalloc(const cs2d_problem *p, const void *dout, int64_t dout_bs, i
  * u, gate (batch, length, dim) of io_dtype, channel stride 1, other strides in elements.  h0 (states, dim) fp32, rows
  * h0_bs apart, or NULL (zeros).  Without `offsets` there are `batch` states.  With them batch is 1 and `offsets`
  * (device, n_seq + 1 ascending int32, or int64 where offsets64 is set) cuts the rows into n_seq sequences
- * [offsets[s], offsets[s+1]) with a state each; a sequence may be empty (its h0 passes through).  Rows of no sequence
- * are not read; y, du and dgate are zero there.  Offsets that do not ascend or leave the tensor set bit 3 of the status
- * word; the outputs are then invalid, nothing outside of them is touched.  At most 2^30 channels and rows, fewer than 2^30
+ * [offsets[s], offsets[s+1]) with a state each; a sequence may be empty (its h0 passes through).  What rows of no sequence
+ * hold does not matter (NaN included), but u, gate and dy must have all `length` rows: they are read; y, du and dgate are
+ * zero there.  Offsets that do not ascend or leave the tensor set bit 3 of the status word; the outputs are then invalid,
+ * nothing outside of them is touched.  At most 2^30 channels and rows, fewer than 2^30
  * sequences: CS2D_ERR_UNSUPPORTED otherwise.
  */
 typedef enum { CS2D_GATE_SIGMOID = 0, CS2D_GATE_LOG = 1, CS2D_GATE_DIRECT = 2 } cs2d_gate_form;

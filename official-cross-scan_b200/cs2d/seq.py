@@ -40,7 +40,8 @@ def gated_scan_1d(u, gate, h0=None, offsets=None, form="sigmoid", weighted=True)
 
     With ``offsets`` (int32 or int64 on the GPU, ``(sequences + 1,)``, ascending) ``u, gate`` are ``(total, dim)`` and sequence ``s``
     is rows ``offsets[s]:offsets[s+1]``; ``h0`` and ``h_last`` are ``(sequences, dim)``.  Sequences may be empty: their state passes
-    through.  Rows of no sequence (padding before the first or behind the last) are not read; ``y`` and the gradients are zero there.
+    through.  What rows of no sequence hold (padding before the first or behind the last) does not matter, NaN included; ``y`` and the
+    gradients are zero there.
     Offsets that do not ascend or leave the tensor are found on the GPU and reported by ``cs2d.device_status()``.
 
     Gradients go to ``u``, ``gate`` and ``h0``, from ``y`` and ``h_last``.  When nothing can ask for one, no state is kept.
