@@ -8,10 +8,10 @@
 //
 // Units are 64 channels wide (rows of 128 bytes of a 16-bit type) or, where those would not fill the GPU, 16 (a warp then holds four slots of rows).
 // Eight warps to a CTA, two CTAs to an SM: one computes while the other waits at its barrier (one CTA of 16 warps: 10 % slower).
-// What bounds it is the issue of instructions, not memory: 24 per element and warp lane in the forward, 49 in the backward (sigmoid gate, ncu),
-// 50 % of the issue slots used, the rest waits for MUFU results, shared memory and the barrier.  Measured (bf16, sigmoid, kernels
-// alone): B16 L16384 D512 forward 184 us, 67 % of the HBM copy rate, backward 360 us, 57 %; B8 L4096 D768 53 + 96 us (192 CTAs on 296 places);
-// B1 L67200 D384 70 + 115 us.
+// What bounds it is the issue of instructions, not memory: 28 per element and warp lane in the forward, 54 in the backward (B8 L4096 D768, sigmoid
+// gate, ncu), 51 % of the issue slots used, the rest waits for MUFU results, shared memory and the barrier.  Measured (bf16, sigmoid, kernels
+// alone): B16 L16384 D512 forward 184 us, 67 % of the HBM copy rate, backward 358 us, 57 % (direct gate, not weighted: 162 us, 76 %, and 315 us, 65 %);
+// B8 L4096 D768 53 + 96 us (192 CTAs on 296 places); B1 L67200 D384 70 + 115 us.
 #pragma once
 
 #include <cooperative_groups.h>
@@ -430,16 +430,18 @@ template <auto KERNEL> cudaError_t start(GScan &P, int G, int rows, size_t smem,
     while (s.wt < NW && (int64_t)s.wt * rows < P.length) s.wt <<= 1;   // the others take further units
     const int64_t tile = (int64_t)s.wt * rows, tiles = (P.length + tile - 1) / tile, per = NW / s.wt, ctas = (P.units + per - 1) / per;
     // The largest cluster of which all fit the GPU at once: a second round would take as long as the first (24 units: 26 clusters of 10
-    // fit, B1 L67200 D384 70 + 115 us; 21 of 12, 90 + 148 us; 33 of 8, 78 + 129 us).
+    // fit, B1 L67200 D384 70 + 114 us; 21 of 12, 88 + 148 us; 33 of 8, 76 + 129 us).
     for (int C = (int)(tiles < MAXC ? tiles : MAXC); C > 1 && s.C == 1; --C)
         if (at_once[dev][C].load(std::memory_order_relaxed) >= ctas) s.C = C;
     s.grid = ctas * s.C;
     configure(cfg, attr, s.grid, s.C, smem, st);
     return cudaLaunchKernelEx(&cfg, KERNEL, (const GScan)P, (const int)s.wt, (const int)s.C);
 }
-// Units of 16 channels instead of 64 where the wide ones would not fill the GPU: rows of 32 bytes instead of 128 are read a little slower (bf16,
-// B16 L16384 D512: 252 + 411 us instead of 184 + 376), but there are four times as many units (B1 L67200 D384: 84 + 150 us instead of 214 + 435;
-// B8 L4096 D768, 96 wide units: 61 + 110 us against 55 + 115).
+// Units of 16 channels instead of 64 where there are few wide ones: rows of 32 bytes instead of 128 take more instructions per element, but there are
+// four times as many units for clusters of at most 16 CTAs.  Wide against narrow, forward + backward in us (bf16, sigmoid): 6 wide units of 67200 rows
+// 86 + 166, 70 + 115; 12 of 16384 37 + 66, 39 + 55; 96 of 4096 53 + 96, 55 + 96; 128 of 16384 184 + 358, 231 + 428.  From 24 to 95 units it depends
+// on the rows: of 512, 64 units 12 + 14, 10 + 14; of 4096, 48 units 31 + 47, 37 + 61; of 16384, 80 units 131 + 247, 180 + 346 (fp32, 48 units of
+// 4096: 47 + 79, 53 + 88).  So the border of 96 is the better one for short rows and not for long ones.
 inline bool narrow(const GScan &P) { return P.batch * (int64_t)((P.dim + 63) / 64) < 96 && P.length > 128; }
 
 }  // namespace gs

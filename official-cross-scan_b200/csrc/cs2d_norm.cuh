@@ -12,9 +12,9 @@
 //
 // A lane holds up to 24 channels: what a row costs beside its channels (addresses, shuffles) is paid once for all of them, and 192 * 2^k channels leave
 // no lane idle.  The backward with a gate and that of images hold 16, since the sums of dw and db take as many registers again (fp32 B25088 D768 gated:
-// 123 us with 8 fp32 channels per lane, 143 with 12).  What bounds it is latency at 16 to 24 warps per SM (128 and 80 registers) and the
-// instructions per row.  Measured: 100352 x 192 bf16 forward 25 us (48 % of the HBM copy rate), backward 41; 25088 x 768 fp32 gated 57 (62 %) and
-// 123 (48 %); B16 D384 128x128 bf16 gated image 147 (63 %) and 328 (47 %).
+// 123 us with 8 fp32 channels per lane, 143 with 12).  What bounds it is latency at 15 to 29 warps per SM (128 to 64 registers; ncu) and the
+// instructions per row.  Measured: 100352 x 192 bf16 forward 25 us (48 % of the HBM copy rate), backward 41 (43 %); 25088 x 768 fp32 gated 57 (62 %)
+// and 123 (48 %); B16 D384 128x128 bf16 gated image 145 (63 %) and 328 (47 %).
 #pragma once
 
 #include <atomic>
